@@ -28,6 +28,8 @@ EXPORTED = (
     "trident_merge_shards", "trident_search_noalloc", "trident_search_prep", "trident_search_seed",
     "trident_search_finish", "trident_workspace_status", "trident_set_wait_limits",
     "trident_noalloc_workspace_bytes", "trident_assign", "trident_stage_y_tensor",
+    "trident_embed_lookup", "trident_embed_grad_workspace_size", "trident_embed_grad", "trident_layer_norm",
+    "trident_layer_norm_grad_workspace_size", "trident_layer_norm_grad", "trident_adamw_step",
 )
 QINFO_LEN = 4
 PHASES = ("coarse", "pairs", "seed", "scan", "merge")
@@ -37,6 +39,11 @@ INDEX_TENSOR_STAGE_Y_ALWAYS = 1
 STATUS_OK = 0
 STATUS_LOCK_TIMEOUT = 1
 STATUS_MMA_TIMEOUT = 2
+STATUS_BAD_ID = 4  # in the status word of an embedding call
+
+# element types and block size of the encoder operators (trident_b200_encoder.h)
+F32, F16, BF16 = 0, 1, 2
+ADAMW_BLOCK = 256
 
 
 def noalloc_workspace_bytes() -> int:
@@ -78,6 +85,37 @@ class TridentIndexDesc(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    """Mirror of `trident_adamw_tensor` (include/trident_b200_encoder.h)."""
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("master", ctypes.c_void_p),
+        ("m", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("m_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+    ]
+
+
+class AdamWConfig(ctypes.Structure):
+    """Mirror of `trident_adamw_config` (include/trident_b200_encoder.h)."""
+    _fields_ = [
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("rounding_seed", ctypes.c_uint32),
+        ("step", ctypes.c_int64),
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("grad_scale", ctypes.c_void_p),
+    ]
+
+
 _LIB = None
 
 
@@ -115,10 +153,20 @@ def lib():
     L.trident_set_wait_limits.argtypes = [i64, i64]
     L.trident_noalloc_workspace_bytes.restype = sz
     L.trident_assign.argtypes = [P, i64, i32, P, P, i32, P, P, P]
+    f32 = ctypes.c_float
+    L.trident_embed_lookup.argtypes = [P, i32, i64, i32, i64, P, i32, i64, f32, P, i64, P, P]
+    L.trident_embed_grad_workspace_size.argtypes = [i64, i64, i32, ctypes.POINTER(sz)]
+    L.trident_embed_grad.argtypes = [P, i32, i64, P, i32, i64, i64, i32, f32, i32, P, i32, i64, P, sz, P, P]
+    L.trident_layer_norm.argtypes = [P, i32, i64, i32, i64, P, P, i32, f32, P, i64, P, P, P]
+    L.trident_layer_norm_grad_workspace_size.argtypes = [i64, i32, ctypes.POINTER(sz)]
+    L.trident_layer_norm_grad.argtypes = [P, i64, P, i64, i32, i64, i32, P, i32, P, P, P, i64, P, P, P, sz, P]
+    L.trident_adamw_step.argtypes = [ctypes.POINTER(AdamWTensor), i32, ctypes.POINTER(AdamWConfig), P]
     for name in ("trident_index_check", "trident_workspace_size", "trident_search", "trident_search_profiled",
                  "trident_coarse", "trident_merge_shards", "trident_search_noalloc", "trident_search_prep",
                  "trident_search_seed", "trident_search_finish", "trident_workspace_status",
-                 "trident_set_wait_limits", "trident_assign"):
+                 "trident_set_wait_limits", "trident_assign", "trident_embed_lookup",
+                 "trident_embed_grad_workspace_size", "trident_embed_grad", "trident_layer_norm",
+                 "trident_layer_norm_grad_workspace_size", "trident_layer_norm_grad", "trident_adamw_step"):
         getattr(L, name).restype = ctypes.c_int
     _LIB = L
     return L

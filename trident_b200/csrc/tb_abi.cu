@@ -14,6 +14,7 @@
 #include <atomic>
 #include <string>
 
+#include "tb_encoder.h"
 #include "tb_internal.h"
 #include "trident_b200.h"
 
@@ -54,6 +55,8 @@ namespace tb {
 static_assert(QI_LEN == TRIDENT_QINFO_LEN, "qinfo layout");
 
 int record_error(int code, const char* msg) { return fail(code, "%s", msg); }
+void count_launches(int n) { g_launches += n; }
+int cuda_status(cudaError_t e, const char* where) { return e == cudaSuccess ? TRIDENT_OK : cuda_fail(e, where); }
 
 uint32_t lock_spin_limit() { return g_lock_spins.load(std::memory_order_relaxed); }
 uint32_t mma_wait_limit() { return g_mma_polls.load(std::memory_order_relaxed); }

@@ -1,0 +1,118 @@
+// Typed wide loads and stores of the encoder operators: N elements of T moved as one 2- to 16-byte
+// access, computed on as float.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tb {
+
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { using type = uint4; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<4> { using type = uint32_t; };
+template <> struct RawOf<2> { using type = uint16_t; };
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Two packed 16-bit elements <-> two floats.
+template <class T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// N elements of T as raw bits. N * sizeof(T) is 2, 4, 8 or 16; addresses are aligned to it.
+template <class T, int N>
+struct Pack {
+    using Raw = typename RawOf<(int)sizeof(T) * N>::type;
+    Raw raw;
+
+    __device__ __forceinline__ static Pack load(const T* p) {
+        Pack r;
+        r.raw = *reinterpret_cast<const Raw*>(p);
+        return r;
+    }
+    // read once: evict first
+    __device__ __forceinline__ static Pack load_stream(const T* p) {
+        Pack r;
+        r.raw = __ldcs(reinterpret_cast<const Raw*>(p));
+        return r;
+    }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+    __device__ __forceinline__ void store_stream(T* p) const { __stcs(reinterpret_cast<Raw*>(p), raw); }
+
+    __device__ __forceinline__ void get(float* f) const {
+        if constexpr (N == 1) {
+            f[0] = to_float(*reinterpret_cast<const T*>(&raw));
+        } else if constexpr (sizeof(T) == 4) {
+            const float* s = reinterpret_cast<const float*>(&raw);
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = s[i];
+        } else {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const float2 t = unpack2<T>(w[i]);
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
+        }
+    }
+    __device__ __forceinline__ static Pack of(const float* f) {
+        Pack r;
+        if constexpr (N == 1) {
+            *reinterpret_cast<T*>(&r.raw) = from_float<T>(f[0]);
+        } else if constexpr (sizeof(T) == 4) {
+            float* s = reinterpret_cast<float*>(&r.raw);
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] = f[i];
+        } else {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&r.raw);
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        }
+        return r;
+    }
+};
+
+// N floats to or from memory of type T, in accesses of at most 16 bytes.
+template <class T, int N>
+__device__ __forceinline__ void load_n(const T* p, float* f) {
+    constexpr int M = (int)sizeof(T) * N > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += M) Pack<T, M>::load(p + i).get(f + i);
+}
+template <class T, int N>
+__device__ __forceinline__ void store_n(T* p, const float* f) {
+    constexpr int M = (int)sizeof(T) * N > 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += M) Pack<T, M>::of(f + i).store(p + i);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+}  // namespace tb
