@@ -57,6 +57,14 @@ void with_vec(int vec, F&& f) {
     f(std::integral_constant<int, 1>{});
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory on the current device (48 KB in all, the kernel's own
+// static memory among them, need no leave).
+template <class K>
+cudaError_t allow_smem(K kernel, size_t bytes) {
+    if (bytes <= 40 * 1024) return cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
 cudaError_t launch_embed_lookup(const void* table, int dtype, int64_t V, int D, int64_t ld, const void* ids, int id64,
                                 int64_t count, float scale, void* out, int64_t ld_out, int32_t* status, cudaStream_t st);
 size_t embed_grad_workspace(int64_t T, int D);

@@ -18,7 +18,6 @@ namespace {
 constexpr int kLaneCols = 32;     // forward: columns of a row that a lane holds
 constexpr int kFwdMaxWarps = 8;   // ... up to 8 warps a row: D <= 8192
 constexpr int kGradCols = 8;      // backward: columns that a thread owns
-constexpr int kGradRows = 4;      // rows in flight in a group
 constexpr int kGradMaxWarps = 16; // D <= 4096
 
 int pow2_at_least(int64_t x) {
@@ -38,6 +37,27 @@ __device__ __forceinline__ float row_sum(float v, float* slot, int warps, int wa
     for (int w = 0; w < warps; ++w) s += slot[w];
     __syncthreads();
     return s;
+}
+
+// A row of D elements at `row` into shared memory, as the 16-byte pieces that hold it: its first element ends
+// up at to + (row & 15). Pieces reach into what lies around the row, but not beyond the `span` bytes from
+// `base` that are the caller's; a piece that would is copied by elements. Thread `i` of `n`.
+template <class T>
+__device__ __forceinline__ void copy_pieces(char* to, const T* row, int D, const T* base, int64_t span, int i, int n) {
+    const char* p = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
+    const char* b = reinterpret_cast<const char*>(base);
+    const char* end = reinterpret_cast<const char*>(row + D);
+    const int pieces = (int)((end - p + 15) >> 4);
+    for (; i < pieces; i += n) {
+        const char* q = p + i * 16;
+        if (q >= b && q + 16 <= b + span) {
+            copy16_async(to + i * 16, q);
+        } else {
+            for (int k = 0; k < 16; k += (int)sizeof(T))
+                if (q + k >= reinterpret_cast<const char*>(row) && q + k < end)
+                    *reinterpret_cast<T*>(to + i * 16 + k) = *reinterpret_cast<const T*>(q + k);
+        }
+    }
 }
 
 // ---- forward
@@ -108,6 +128,267 @@ __global__ void __launch_bounds__(256) norm_kernel(const T* x, int64_t rows, int
     }
 }
 
+// Many rows of 16-byte columns. Warps stay and take turns of ROWS rows; the next rows are on their way into
+// shared memory (each lane copies the columns that it will use, so no barrier is needed) while some are
+// computed, and weight and bias wait in shared memory as float, read once for ROWS rows. LANES lanes a row
+// for narrow rows, else `warps` warps.
+constexpr int kStages = 3;
+constexpr int kRowWarps = 16;  // warps of a block
+
+template <int NV> constexpr int kRowsAtOnce = NV >= 4 ? 1 : NV == 2 ? 2 : 4;
+
+template <class T, class P, int NV, int LANES>
+__global__ void __launch_bounds__(32 * kRowWarps) norm_rows_kernel(const T* x, int64_t rows, int D, int64_t ld_x,
+                                                                   const P* __restrict__ w, const P* __restrict__ b,
+                                                                   float eps, T* y, int64_t ld_y, float* mean, float* rstd,
+                                                                   int warps) {
+    constexpr int VEC = 16 / (int)sizeof(T), H = VEC / 2, ROWS = kRowsAtOnce<NV>;
+    extern __shared__ __align__(16) uint4 smem[];
+    __shared__ float slots[2][kRowWarps][ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int in_row = LANES < 32 ? 0 : warp % warps;
+    const int group = LANES < 32 ? threadIdx.x / LANES : warp / warps;
+    const int groups = LANES < 32 ? kRowWarps * (32 / LANES) : kRowWarps / warps;
+    const int sub = lane & (LANES - 1);
+    const int cols = D / VEC;
+    const float inv_d = 1.0f / (float)D;
+    uint4* ring = smem + warp * (kStages * ROWS * NV * 32) + lane;  // [stage][row][k][lane of the warp]
+    float4* pw = reinterpret_cast<float4*>(smem + kRowWarps * kStages * ROWS * NV * 32);  // [half][column] of 4 floats
+    float4* pb = pw + (VEC / 4) * cols;
+    for (int i = threadIdx.x; i < (VEC / 4) * cols; i += blockDim.x) {
+        const int h = i / cols, c = i - h * cols;
+        float f[4] = {1.0f, 1.0f, 1.0f, 1.0f}, g[4] = {};
+        if (w) load_n<P, 4>(w + (int64_t)c * VEC + h * 4, f);
+        if (b) load_n<P, 4>(b + (int64_t)c * VEC + h * 4, g);
+        pw[i] = make_float4(f[0], f[1], f[2], f[3]);
+        pb[i] = make_float4(g[0], g[1], g[2], g[3]);
+    }
+    const int col0 = in_row * LANES + sub, col_step = warps * LANES;
+    bool on[NV];  // columns past the end read as 0 and are kept 0
+#pragma unroll
+    for (int k = 0; k < NV; ++k) on[k] = col0 + k * col_step < cols;
+    const int64_t stride = (int64_t)gridDim.x * groups * ROWS;
+    const int steps = (int)((rows + stride - 1) / stride);  // the same for every group
+    int64_t row = ((int64_t)blockIdx.x * groups + group) * ROWS;
+    int64_t ahead = row;                       // first row of the next copy
+    const T* src = x + row * ld_x + (int64_t)col0 * VEC;
+    int fetch_at = 0, take_at = 0;             // stages
+    auto fetch = [&]() {
+        const int64_t left = rows - ahead;
+        uint4* to = ring + fetch_at * (ROWS * NV * 32);
+        const T* p = src;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                copy16_async_or_zero(to + (r * NV + k) * 32, r < left && on[k] ? p + k * col_step * VEC : x, r < left && on[k]);
+            p += ld_x;
+        }
+        copy_commit();
+        ahead += stride;
+        src += stride * ld_x;
+        fetch_at = fetch_at + 1 == kStages ? 0 : fetch_at + 1;
+    };
+#pragma unroll
+    for (int t = 0; t < kStages - 1; ++t) fetch();
+    __syncthreads();  // weight and bias
+    auto sums = [&](float* v, int which) {  // over the row, of ROWS values
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) v[r] += __shfl_xor_sync(0xffffffffu, v[r], o);
+        }
+        if (LANES < 32 || warps == 1) return;
+        if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) slots[which][warp][r] = v[r];
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(warps * 32) : "memory");
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) v[r] = 0.0f;
+        for (int q = 0; q < warps; ++q) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) v[r] += slots[which][group * warps + q][r];
+        }
+    };
+    T* dst = y + row * ld_y + (int64_t)col0 * VEC;
+    for (int t = 0; t < steps; ++t) {
+        fetch();
+        copy_wait<kStages - 1>();
+        const uint4* from = ring + take_at * (ROWS * NV * 32);
+        const int64_t left = rows - row;  // rows past the end compute on old copies and are not stored
+        float2 f[ROWS][NV][H];
+        float v[ROWS], mu[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float2 s = splat(0.0f);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                unpack16<T>(from[(r * NV + k) * 32], f[r][k]);
+#pragma unroll
+                for (int i = 0; i < H; ++i) s = __fadd2_rn(s, f[r][k][i]);
+            }
+            v[r] = s.x + s.y;
+        }
+        sums(v, 0);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            mu[r] = v[r] * inv_d;
+            float2 s = splat(0.0f);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const float2 shift = splat(on[k] ? -mu[r] : 0.0f);
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    f[r][k][i] = __fadd2_rn(f[r][k][i], shift);
+                    s = __ffma2_rn(f[r][k][i], f[r][k][i], s);
+                }
+            }
+            v[r] = s.x + s.y;
+        }
+        sums(v, 1);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) v[r] = rsqrtf(fmaf(v[r], inv_d, eps));
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = on[k] ? col0 + k * col_step : 0;
+#pragma unroll
+            for (int h = 0; h < VEC / 4; ++h) {
+                const float4 wv = pw[h * cols + c], bv = pb[h * cols + c];
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    float2* g = f[r][k] + 2 * h;
+                    g[0] = __ffma2_rn(__fmul2_rn(g[0], splat(v[r])), make_float2(wv.x, wv.y), make_float2(bv.x, bv.y));
+                    g[1] = __ffma2_rn(__fmul2_rn(g[1], splat(v[r])), make_float2(wv.z, wv.w), make_float2(bv.z, bv.w));
+                }
+            }
+        }
+        T* q = dst;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            if (r < left) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                    if (on[k]) __stcs(reinterpret_cast<uint4*>(q + k * col_step * VEC), pack16<T>(f[r][k]));
+                if (in_row == 0 && sub == 0) {
+                    if (mean) mean[row + r] = mu[r];
+                    if (rstd) rstd[row + r] = v[r];
+                }
+            }
+            q += ld_y;
+        }
+        row += stride;
+        dst += stride * ld_y;
+        take_at = take_at + 1 == kStages ? 0 : take_at + 1;
+    }
+}
+
+// Rows that start anywhere: as norm_rows_kernel, but the warps of a row copy the 16-byte pieces that hold it and
+// read their columns E at a time (2 where rows of a 16-bit type start at 4-byte places). NV such reads a lane.
+template <class T, class P, int E, int NV, int S>
+__global__ void __launch_bounds__(32 * kRowWarps) norm_ragged_kernel(const T* x, int64_t rows, int D, int64_t ld_x,
+                                                                     const P* __restrict__ w, const P* __restrict__ b,
+                                                                     float eps, T* y, int64_t ld_y, float* mean, float* rstd,
+                                                                     int warps, int slot_bytes) {
+    constexpr int N = E * NV, H = N / 2;  // columns and pairs of columns of a lane
+    extern __shared__ __align__(16) uint4 smem[];
+    __shared__ float slots[2][kRowWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_row = warp % warps, group = warp / warps;
+    const int groups = kRowWarps / warps;
+    const float inv_d = 1.0f / (float)D;
+    char* ring = reinterpret_cast<char*>(smem) + group * S * slot_bytes;
+    float* pw = reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + groups * S * slot_bytes);
+    float* pb = pw + D;
+    for (int i = threadIdx.x; i < D; i += blockDim.x) {
+        pw[i] = w ? to_float(w[i]) : 1.0f;
+        pb[i] = b ? to_float(b[i]) : 0.0f;
+    }
+    const int col0 = in_row * 32 * N + lane * E;  // a lane's column j: col0 + j / E * 32 * E + j % E
+    const bool full = (in_row + 1) * 32 * N <= D;
+    auto on = [&](int j) { return col0 + j / E * 32 * E + j % E < D; };
+    const int64_t stride = (int64_t)gridDim.x * groups;
+    const int steps = (int)((rows + stride - 1) / stride);  // the same for every group
+    int64_t row = (int64_t)blockIdx.x * groups + group, ahead = row;
+    const int64_t span = ((rows - 1) * ld_x + D) * (int64_t)sizeof(T);
+    int fetch_at = 0, take_at = 0;
+    auto fetch = [&]() {
+        if (ahead < rows) copy_pieces(ring + fetch_at * slot_bytes, x + ahead * ld_x, D, x, span, in_row * 32 + lane, warps * 32);
+        copy_commit();
+        ahead += stride;
+        fetch_at = fetch_at + 1 == S ? 0 : fetch_at + 1;
+    };
+    auto barrier = [&]() {
+        if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(warps * 32) : "memory");
+        else __syncwarp();
+    };
+    auto sum = [&](float v, int which) {
+        v = warp_sum(v);
+        if (warps == 1) return v;
+        if (lane == 0) slots[which][warp] = v;
+        barrier();
+        float r = 0.0f;
+        for (int q = 0; q < warps; ++q) r += slots[which][group * warps + q];
+        return r;
+    };
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t) fetch();
+    __syncthreads();  // weight and bias
+    for (int t = 0; t < steps; ++t) {
+        copy_wait<S - 2>();
+        barrier();  // the row is there for all its warps, and the stage before is free
+        fetch();
+        auto compute = [&](auto mask) {
+            constexpr bool MASK = decltype(mask)::value;
+            const T* q = reinterpret_cast<const T*>(ring + take_at * slot_bytes + (reinterpret_cast<uintptr_t>(x + row * ld_x) & 15)) + col0;
+            float2 f[H];
+            float2 s = splat(0.0f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                if constexpr (E == 2) {
+                    f[i] = !MASK || on(2 * i) ? unpack2<T>(*reinterpret_cast<const uint32_t*>(q + 64 * i)) : splat(0.0f);
+                } else {
+                    f[i].x = !MASK || on(2 * i) ? to_float(q[64 * i]) : 0.0f;
+                    f[i].y = !MASK || on(2 * i + 1) ? to_float(q[64 * i + 32]) : 0.0f;
+                }
+                s = __fadd2_rn(s, f[i]);
+            }
+            const float mu = sum(s.x + s.y, 0) * inv_d;
+            s = splat(0.0f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                f[i] = __fadd2_rn(f[i], MASK ? make_float2(on(2 * i) ? -mu : 0.0f, on(2 * i + 1) ? -mu : 0.0f) : splat(-mu));
+                s = __ffma2_rn(f[i], f[i], s);
+            }
+            const float r = rsqrtf(fmaf(sum(s.x + s.y, 1), inv_d, eps));
+            T* o = y + row * ld_y + col0;
+            if (row < rows) {
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const int a = 64 * i, c = E == 2 ? a + 1 : a + 32;
+                    const bool oa = !MASK || on(2 * i), ob = !MASK || on(2 * i + 1);
+                    const float2 wv = make_float2(oa ? pw[col0 + a] : 0.0f, ob ? pw[col0 + c] : 0.0f);
+                    const float2 bv = make_float2(oa ? pb[col0 + a] : 0.0f, ob ? pb[col0 + c] : 0.0f);
+                    f[i] = __ffma2_rn(__fmul2_rn(f[i], splat(r)), wv, bv);
+                    if constexpr (E == 2) {
+                        if (oa) *reinterpret_cast<uint32_t*>(o + a) = pack2<T>(f[i].x, f[i].y);
+                    } else {
+                        if (oa) o[a] = from_float<T>(f[i].x);
+                        if (ob) o[c] = from_float<T>(f[i].y);
+                    }
+                }
+                if (in_row == 0 && lane == 0) {
+                    if (mean) mean[row] = mu;
+                    if (rstd) rstd[row] = r;
+                }
+            }
+        };
+        if (full) compute(std::false_type{});
+        else compute(std::true_type{});
+        row += stride;
+        take_at = take_at + 1 == S ? 0 : take_at + 1;
+    }
+}
+
 // Any D: one block a row, the row read once for each of the three steps (from L2 after the first).
 template <class T, class P>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const T* x, int64_t rows, int D, int64_t ld_x, const P* __restrict__ w,
@@ -154,6 +435,59 @@ cudaError_t norm_typed(const T* x, int64_t rows, int D, int64_t ld_x, const P* w
     if (vec < kVec) vec = 1;
     const int per_warp = kLaneCols * 32;
     const int warps = pow2_at_least((D + per_warp - 1) / per_warp);
+    if (vec == kVec && rows * warps >= (int64_t)num_sms() * kRowWarps * 8) {
+        // 32 columns a lane (16 of a float32 row that takes more than one warp, for shared memory)
+        const int wide = D <= per_warp || sizeof(T) == 2 ? per_warp : per_warp / 2;
+        const int row_warps = pow2_at_least((D + wide - 1) / wide);
+        auto stream = [&](auto k, auto l) {
+            constexpr int NV = decltype(k)::value, LANES = decltype(l)::value;
+            const size_t bytes = (size_t)kRowWarps * kStages * kRowsAtOnce<NV> * NV * 32 * 16 + (size_t)D * 8;
+            const cudaError_t e = allow_smem(norm_rows_kernel<T, P, NV, LANES>, bytes);
+            if (e != cudaSuccess) return e;
+            const int per_sm = bytes <= 112 * 1024 ? 2 : 1;  // of 227 KB, 1 KB a block the system's
+            norm_rows_kernel<T, P, NV, LANES><<<num_sms() * per_sm, 32 * kRowWarps, bytes, st>>>(x, rows, D, ld_x, w, b, eps, y,
+                                                                                               ld_y, mean, rstd, row_warps);
+            return cudaGetLastError();
+        };
+        const int cols = D / kVec, n = (cols + 32 * row_warps - 1) / (32 * row_warps);
+        const std::integral_constant<int, 32> all;
+        if (cols <= 8) return stream(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+        if (cols <= 16) return stream(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+        if (n == 1) return stream(std::integral_constant<int, 1>{}, all);
+        if (n == 2) return stream(std::integral_constant<int, 2>{}, all);
+        if constexpr (kVec == 4)
+            if (n > 4) return stream(std::integral_constant<int, 8>{}, all);
+        return stream(std::integral_constant<int, 4>{}, all);
+    }
+    if (vec < kVec && rows * warps >= (int64_t)num_sms() * kRowWarps * 2) {
+        const int es = (int)sizeof(T), slot = (D * es / 16 + 2) * 16;
+        auto stream = [&](auto e_, auto k, auto s_) {
+            constexpr int E = decltype(e_)::value, NV = decltype(k)::value, S = decltype(s_)::value;
+            const size_t bytes = (size_t)(kRowWarps / warps) * S * slot + (size_t)D * 8;
+            const cudaError_t e = allow_smem(norm_ragged_kernel<T, P, E, NV, S>, bytes);
+            if (e != cudaSuccess) return e;
+            const int per_sm = bytes <= 112 * 1024 ? 2 : 1;
+            norm_ragged_kernel<T, P, E, NV, S><<<num_sms() * per_sm, 32 * kRowWarps, bytes, st>>>(x, rows, D, ld_x, w, b, eps, y, ld_y,
+                                                                                                mean, rstd, warps, slot);
+            return cudaGetLastError();
+        };
+        const int lane_cols = (D + 32 * warps - 1) / (32 * warps);
+        auto pick = [&](auto e_) {
+            constexpr int E = decltype(e_)::value;
+            const std::integral_constant<int, 3> s3;
+            if (lane_cols <= 4) return stream(e_, std::integral_constant<int, 4 / E>{}, s3);
+            if (lane_cols <= 8) return stream(e_, std::integral_constant<int, 8 / E>{}, s3);
+            if (lane_cols <= 16) return stream(e_, std::integral_constant<int, 16 / E>{}, s3);
+            if constexpr (sizeof(T) == 4)  // the widest rows and their weights leave room for two stages
+                if (D > 4096) return stream(e_, std::integral_constant<int, 32 / E>{}, std::integral_constant<int, 2>{});
+            return stream(e_, std::integral_constant<int, 32 / E>{}, s3);
+        };
+        if constexpr (sizeof(T) == 2) {
+            const int pair = wide_elements({{x, ld_x, 2}, {y, ld_y, 2}}, D, 2);
+            if (pair == 2) return pick(std::integral_constant<int, 2>{});
+        }
+        return pick(std::integral_constant<int, 1>{});
+    }
     const int64_t per_block = 8 / warps;
     const int64_t grid = (rows + per_block - 1) / per_block;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -182,113 +516,273 @@ cudaError_t norm_typed(const T* x, int64_t rows, int D, int64_t ld_x, const P* w
 
 // ---- backward
 
-// Groups of `warps` warps take turns of kGradRows rows; NV * VEC = kGradCols columns a thread.
-template <class T, class P, int VEC>
-__global__ void __launch_bounds__(32 * kGradMaxWarps) norm_grad_kernel(const T* dy, int64_t ld_dy, const T* __restrict__ x, int64_t ld_x, int64_t rows, int D,
-                                 const P* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
-                                 T* dx, int64_t ld_dx, float* __restrict__ part, int64_t ld_part, int warps) {
-    constexpr int NV = kGradCols / VEC;
-    __shared__ float2 slots[2][kGradMaxWarps][kGradRows];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int in_row = warp % warps, group = warp / warps;
-    const int groups_here = blockDim.x / 32 / warps;
-    const int64_t groups = (int64_t)gridDim.x * groups_here, me = (int64_t)blockIdx.x * groups_here + group;
-    const int cols = D / VEC;
+// One pass over x and dy: groups of LANES lanes (a narrow row) or of `warps` warps take turns of R rows.
+// A thread owns kGradCols columns for all rows of its group. The next rows are on their way into shared
+// memory while one set is computed, so that the loads in flight take no registers:
+//   E = 0: rows of whole 16-byte columns; each thread copies its own columns and needs no barrier for them;
+//   E = 1, 2: rows that start anywhere; the group copies the 16-byte pieces that hold them, and a thread's
+//          columns are read E at a time (2 where rows of a 16-bit type start at 4-byte places).
+template <class T, class P, int R, int LANES, int E, int S>
+__global__ void __launch_bounds__(32 * kGradMaxWarps)
+    norm_grad_rows_kernel(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int64_t rows, int D, const P* __restrict__ w,
+                          const float* __restrict__ mean, const float* __restrict__ rstd, T* dx, int64_t ld_dx,
+                          float* __restrict__ part, int64_t ld_part, int warps, int slot_bytes) {
+    constexpr int VEC = 16 / (int)sizeof(T), NV = kGradCols / VEC, N = kGradCols / 2;  // N pairs of columns
+    constexpr int PER = 32 / LANES;
+    extern __shared__ __align__(16) uint4 smem[];
+    __shared__ __align__(16) float slots[2][kGradMaxWarps * PER][2 * R];
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, sub = lane & (LANES - 1);
+    const int in_row = warp % warps, warp_group = warp / warps;
+    const int group = LANES < 32 ? tid / LANES : warp_group;
+    const int groups_here = threads / 32 / warps * PER;
     const float inv_d = 1.0f / (float)D;
-    int col[NV];
-    float wf[kGradCols], dw[kGradCols] = {}, db[kGradCols] = {};
+    // column of element j of this thread
+    auto column = [&](int j) {
+        if constexpr (E == 0) return ((j / VEC * warps + in_row) * LANES + sub) * VEC + j % VEC;
+        if constexpr (E == 2) return ((in_row * N + j / 2) * 32 + lane) * 2 + j % 2;
+        return (in_row * kGradCols + j) * 32 + lane;
+    };
+    const bool full = (in_row + 1) * 32 * kGradCols <= D;   // E != 0: no column of this warp is past the end
+    const bool flat = ld_x == D && ld_dy == D;              // the rows of a step are one piece of memory
+    float2 wf[N], dw[N], db[N];
+    bool on[kGradCols];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        col[k] = (k * warps + in_row) * 32 + lane;
+    for (int i = 0; i < N; ++i) {
+        float f[2];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) wf[k * VEC + i] = 1.0f;
-        if (w && col[k] < cols) load_n<P, VEC>(w + (int64_t)col[k] * VEC, wf + k * VEC);
+        for (int h = 0; h < 2; ++h) {
+            const int c = column(2 * i + h);
+            on[2 * i + h] = c < D;
+            f[h] = w && c < D ? to_float(w[c]) : 1.0f;
+        }
+        wf[i] = make_float2(f[0], f[1]);
+        dw[i] = db[i] = splat(0.0f);
     }
-    const int64_t steps = (rows + groups * kGradRows - 1) / (groups * kGradRows);  // the same for every group
-    for (int64_t t = 0; t < steps; ++t) {
-        const int64_t r0 = (t * groups + me) * kGradRows;
-        Pack<T, VEC> px[kGradRows][NV], pg[kGradRows][NV];
-        float mu[kGradRows], rs[kGradRows];
-#pragma unroll
-        for (int r = 0; r < kGradRows; ++r) {
-            if (r0 + r >= rows) continue;
-            mu[r] = mean[r0 + r];
-            rs[r] = rstd[r0 + r];
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (col[k] >= cols) continue;
-                px[r][k] = Pack<T, VEC>::load(x + (r0 + r) * ld_x + (int64_t)col[k] * VEC);
-                pg[r][k] = Pack<T, VEC>::load(dy + (r0 + r) * ld_dy + (int64_t)col[k] * VEC);
-            }
+    const int64_t stride = (int64_t)gridDim.x * groups_here * R;
+    const int steps = (int)((rows + stride - 1) / stride);  // the same for every group
+    int64_t row = ((int64_t)blockIdx.x * groups_here + group) * R, ahead = row;
+    const T *px = x + row * ld_x, *pg = dy + row * ld_dy;   // of the next copy
+    const int64_t span_x = ((rows - 1) * ld_x + D) * (int64_t)sizeof(T), span_g = ((rows - 1) * ld_dy + D) * (int64_t)sizeof(T);
+    constexpr int kStage = R * 2 * NV;  // E = 0: [row][x, dy][k] of [thread]
+    int fetch_at = 0, take_at = 0;
+    auto fetch = [&]() {
+        const int64_t left = rows - ahead;
+        const T *qx = px, *qg = pg;
+        char* slot = reinterpret_cast<char*>(smem) + (fetch_at * groups_here + group) * R * 2 * slot_bytes;
+        if (E != 0 && flat && left > 0) {
+            const int n = (int)(left < R ? left : R) * D;
+            copy_pieces(slot, qx, n, x, span_x, in_row * 32 + lane, warps * 32);
+            copy_pieces(slot + R * slot_bytes, qg, n, dy, span_g, in_row * 32 + lane, warps * 32);
         }
-        float s1[kGradRows], s2[kGradRows];
 #pragma unroll
-        for (int r = 0; r < kGradRows; ++r) {
-            s1[r] = s2[r] = 0.0f;
-            if (r0 + r >= rows) continue;
+        for (int r = 0; r < R; ++r) {
+            if constexpr (E == 0) {
+                uint4* to = smem + fetch_at * kStage * threads + tid;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (col[k] >= cols) continue;
-                float xf[VEC], gf[VEC];
-                px[r][k].get(xf);
-                pg[r][k].get(gf);
+                for (int k = 0; k < NV; ++k) {  // 0 in columns and rows past the end: they add nothing
+                    const bool there = r < left && on[k * VEC];
+                    copy16_async_or_zero(to + ((r * 2) * NV + k) * threads, there ? qx + column(k * VEC) : x, there);
+                    copy16_async_or_zero(to + ((r * 2 + 1) * NV + k) * threads, there ? qg + column(k * VEC) : dy, there);
+                }
+            } else if (r < left && !flat) {
+                copy_pieces(slot + r * slot_bytes, qx, D, x, span_x, in_row * 32 + lane, warps * 32);
+                copy_pieces(slot + (R + r) * slot_bytes, qg, D, dy, span_g, in_row * 32 + lane, warps * 32);
+            }
+            qx += ld_x;
+            qg += ld_dy;
+        }
+        copy_commit();
+        ahead += stride;
+        px += stride * ld_x;
+        pg += stride * ld_dy;
+        fetch_at = fetch_at + 1 == S ? 0 : fetch_at + 1;
+    };
+    auto group_barrier = [&]() {
+        if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + warp_group), "r"(warps * 32) : "memory");
+        else __syncwarp();
+    };
+    // this thread's columns of row r of the stage in hand; `at`: where the row (flat: the step's first row)
+    // lies in memory. With MASK 0 past the end.
+    auto take = [&](int r, bool is_dy, const T* at, float2* f, auto mask) {
+        [[maybe_unused]] constexpr bool MASK = decltype(mask)::value;
+        if constexpr (E == 0) {
+            const uint4* from = smem + take_at * kStage * threads + tid;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float xh = (xf[i] - mu[r]) * rs[r];
-                    const float g = gf[i] * wf[k * VEC + i];
-                    dw[k * VEC + i] = fmaf(gf[i], xh, dw[k * VEC + i]);
-                    db[k * VEC + i] += gf[i];
-                    s1[r] += g;
-                    s2[r] = fmaf(g, xh, s2[r]);
+            for (int k = 0; k < NV; ++k) unpack16<T>(from[((r * 2 + is_dy) * NV + k) * threads], f + k * (VEC / 2));
+        } else {
+            const char* slot = reinterpret_cast<const char*>(smem) + ((take_at * groups_here + group) * 2 + is_dy) * R * slot_bytes;
+            const T* q = reinterpret_cast<const T*>(slot + (reinterpret_cast<uintptr_t>(at) & 15) + (flat ? r * D * (int)sizeof(T) : r * slot_bytes)) + column(0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if constexpr (E == 2) {
+                    f[i] = !MASK || on[2 * i] ? unpack2<T>(*reinterpret_cast<const uint32_t*>(q + 64 * i)) : splat(0.0f);
+                } else {
+                    f[i].x = !MASK || on[2 * i] ? to_float(q[64 * i]) : 0.0f;
+                    f[i].y = !MASK || on[2 * i + 1] ? to_float(q[64 * i + 32]) : 0.0f;
                 }
             }
         }
+    };
 #pragma unroll
-        for (int r = 0; r < kGradRows; ++r) {
-            s1[r] = warp_sum(s1[r]);
-            s2[r] = warp_sum(s2[r]);
-        }
-        if (warps > 1) {  // two sets of slots in turn: one barrier a step
-            if (lane == 0) {
+    for (int t = 0; t < S - 1; ++t) fetch();
+    const bool wide = ((reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) & (4 * R - 1)) == 0;
+    float rs_next[R], mu_next[R];  // the statistics of the step after
+    auto stats = [&](int64_t at) {
+        if (wide && at + R <= rows) {
+            Pack<float, R>::load(rstd + at).get(rs_next);
+            Pack<float, R>::load(mean + at).get(mu_next);
+        } else {
 #pragma unroll
-                for (int r = 0; r < kGradRows; ++r) slots[t & 1][warp][r] = make_float2(s1[r], s2[r]);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < kGradRows; ++r) {
-                s1[r] = s2[r] = 0.0f;
-                for (int q = 0; q < warps; ++q) {
-                    const float2 v = slots[t & 1][group * warps + q][r];
-                    s1[r] += v.x;
-                    s2[r] += v.y;
-                }
+            for (int r = 0; r < R; ++r) {
+                rs_next[r] = at + r < rows ? rstd[at + r] : 0.0f;
+                mu_next[r] = at + r < rows ? mean[at + r] : 0.0f;
             }
         }
+    };
+    stats(row);
+    T* out = dx + row * ld_dx;
+    const T *xr = x + row * ld_x, *gr = dy + row * ld_dy;
+    for (int t = 0; t < steps; ++t) {
+        copy_wait<S - 2>();
+        if constexpr (E != 0) group_barrier();  // the rows are there for all, and the stage before is free
+        fetch();
+        const int left = (int)min(rows - row, (int64_t)R);  // may be negative
+        float rs[R], mu[R];
 #pragma unroll
-        for (int r = 0; r < kGradRows; ++r) {
-            if (r0 + r >= rows) continue;
-            const float c1 = s1[r] * inv_d, c2 = s2[r] * inv_d;
+        for (int r = 0; r < R; ++r) {
+            rs[r] = rs_next[r];
+            mu[r] = -mu_next[r];
+        }
+        stats(row + stride);
+        float v[2 * R];  // sums of g, then of g (x - mean), over this thread's columns
+        auto first = [&](auto mask) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (col[k] >= cols) continue;
-                float xf[VEC], gf[VEC];
-                px[r][k].get(xf);
-                pg[r][k].get(gf);
+            for (int r = 0; r < R; ++r) {
+                float2 s1 = splat(0.0f), s2 = splat(0.0f);
+                if (E == 0 || r < left) {
+                    float2 xf[N], gf[N];
+                    take(r, false, flat ? xr : xr + r * ld_x, xf, mask);
+                    take(r, true, flat ? gr : gr + r * ld_dy, gf, mask);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float xh = (xf[i] - mu[r]) * rs[r];
-                    gf[i] = rs[r] * (gf[i] * wf[k * VEC + i] - c1 - xh * c2);
+                    for (int i = 0; i < N; ++i) {
+                        const float2 d = __fadd2_rn(xf[i], splat(mu[r]));
+                        const float2 g = __fmul2_rn(gf[i], wf[i]);
+                        dw[i] = __ffma2_rn(__fmul2_rn(gf[i], splat(rs[r])), d, dw[i]);
+                        db[i] = __fadd2_rn(db[i], gf[i]);
+                        s1 = __fadd2_rn(s1, g);
+                        s2 = __ffma2_rn(g, d, s2);
+                    }
                 }
-                Pack<T, VEC>::of(gf).store(dx + (r0 + r) * ld_dx + (int64_t)col[k] * VEC);
+                v[r] = s1.x + s1.y;
+                v[R + r] = s2.x + s2.y;
             }
+        };
+        if (E == 0 || full) first(std::false_type{});
+        else first(std::true_type{});
+        // 2 R sums over the lanes together: each step halves the sums that a lane holds, or adds a pair of lanes
+        int mine = 0;
+#pragma unroll
+        for (int o = LANES / 2, m = 2 * R; o > 0; o >>= 1) {
+            if (m > 1) {
+                m /= 2;
+                const bool up = lane & o;
+#pragma unroll
+                for (int i = 0; i < m; ++i) {
+                    const float keep = up ? v[i + m] : v[i], give = up ? v[i] : v[i + m];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+                mine = mine * 2 + (up ? 1 : 0);
+            } else {
+                v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+            }
+        }
+        // two sets of slots in turn: one barrier a step
+        if ((lane & (LANES / (2 * R) - 1)) == 0) slots[t & 1][LANES < 32 ? group : warp][mine] = v[0];
+        group_barrier();
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) v[i] = 0.0f;
+        for (int q = 0; q < warps; ++q) {
+            const float4* sq = reinterpret_cast<const float4*>(slots[t & 1][LANES < 32 ? group : warp_group * warps + q]);
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i) {
+                const float4 f = sq[i];
+                v[4 * i] += f.x;
+                v[4 * i + 1] += f.y;
+                v[4 * i + 2] += f.z;
+                v[4 * i + 3] += f.w;
+            }
+        }
+        T* q = out;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float c1 = -v[r] * inv_d * rs[r], c2 = -v[R + r] * inv_d * rs[r] * rs[r] * rs[r];
+            if (E == 0 || r < left) {
+                float2 xf[N], gf[N];
+                take(r, false, flat ? xr : xr + r * ld_x, xf, std::false_type{});  // columns past the end are not stored
+                take(r, true, flat ? gr : gr + r * ld_dy, gf, std::false_type{});
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float2 d = __fadd2_rn(xf[i], splat(mu[r]));
+                    const float2 g = __fmul2_rn(gf[i], wf[i]);
+                    gf[i] = __ffma2_rn(d, splat(c2), __ffma2_rn(g, splat(rs[r]), splat(c1)));
+                }
+                if constexpr (E == 0) {
+#pragma unroll
+                    for (int k = 0; k < NV; ++k)
+                        if (r < left && on[k * VEC]) __stcs(reinterpret_cast<uint4*>(q + column(k * VEC)), pack16<T>(gf + k * (VEC / 2)));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        if constexpr (E == 2) {
+                            if (on[2 * i]) *reinterpret_cast<uint32_t*>(q + column(2 * i)) = pack2<T>(gf[i].x, gf[i].y);
+                        } else {
+                            if (on[2 * i]) q[column(2 * i)] = from_float<T>(gf[i].x);
+                            if (on[2 * i + 1]) q[column(2 * i + 1)] = from_float<T>(gf[i].y);
+                        }
+                    }
+                }
+            }
+            q += ld_dx;
+        }
+        row += stride;
+        out += stride * ld_dx;
+        xr += stride * ld_x;
+        gr += stride * ld_dy;
+        take_at = take_at + 1 == S ? 0 : take_at + 1;
+    }
+    // one partial row a block: the lanes with the same columns, then the block's groups in order
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
+            dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
+            db[i].x += __shfl_xor_sync(0xffffffffu, db[i].x, o);
+            db[i].y += __shfl_xor_sync(0xffffffffu, db[i].y, o);
         }
     }
-    float* pw = part + me * 2 * ld_part;
+    const int sets = threads / 32 / warps;
+    float* to = part + (int64_t)blockIdx.x * 2 * ld_part;
+    if (sets > 1) {
+        copy_wait<0>();
+        __syncthreads();  // the copies' memory is free
+        to = reinterpret_cast<float*>(smem) + warp_group * 2 * D;
+    }
+    const int64_t second = sets > 1 ? D : ld_part;
+    if (lane < LANES) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        if (col[k] >= cols) continue;
-        store_n<float, VEC>(pw + (int64_t)col[k] * VEC, dw + k * VEC);
-        store_n<float, VEC>(pw + ld_part + (int64_t)col[k] * VEC, db + k * VEC);
+        for (int j = 0; j < kGradCols; ++j) {
+            if (!on[j]) continue;
+            to[column(j)] = j % 2 ? dw[j / 2].y : dw[j / 2].x;
+            to[second + column(j)] = j % 2 ? db[j / 2].y : db[j / 2].x;
+        }
+    }
+    if (sets == 1) return;
+    __syncthreads();
+    for (int i = tid; i < 2 * D; i += threads) {
+        float a = 0.0f;
+        for (int g = 0; g < sets; ++g) a += reinterpret_cast<const float*>(smem)[g * 2 * D + i];
+        part[((int64_t)blockIdx.x * 2 + (i >= D)) * ld_part + (i >= D ? i - D : i)] = a;
     }
 }
 
@@ -363,8 +857,7 @@ constexpr int kLongParts = 64;  // partial rows of the any-D path
 struct GradShape {
     int warps;         // warps a row; 0: the any-D path
     int threads;
-    int blocks;
-    int64_t parts;     // partial rows
+    int64_t parts;     // partial rows, one a block, at most
     int64_t ld_part;
 };
 
@@ -373,25 +866,22 @@ GradShape grad_shape(int64_t rows, int D) {
     g.ld_part = (D + 3) / 4 * 4;
     const int per_warp = 32 * kGradCols;
     if (D > per_warp * kGradMaxWarps) {
-        g.warps = g.threads = g.blocks = 0;
+        g.warps = g.threads = 0;
         g.parts = rows < kLongParts ? rows : kLongParts;
         return g;
     }
     g.warps = pow2_at_least((D + per_warp - 1) / per_warp);
-    g.threads = g.warps * 32 < 128 ? 128 : g.warps * 32;
-    const int groups = g.threads / 32 / g.warps;
-    // four 128-thread blocks an SM at this kernel's registers; one step of kGradRows rows a group at least
-    const int64_t most = (int64_t)num_sms() * (512 / g.threads > 0 ? 512 / g.threads : 1);
-    const int64_t need = (rows + (int64_t)groups * kGradRows - 1) / ((int64_t)groups * kGradRows);
-    g.blocks = (int)(need < most ? need : most);
-    g.parts = (int64_t)g.blocks * groups;
+    g.threads = g.warps <= 8 ? 256 : g.warps * 32;
+    // 512 threads an SM at this kernel's registers; a row of its own for each block at least
+    const int64_t most = (int64_t)num_sms() * (512 / g.threads);
+    g.parts = rows < most ? rows : most;
     return g;
 }
 
 template <class T, class P>
 cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int64_t rows, int D, const P* w, const float* mean,
                        const float* rstd, T* dx, int64_t ld_dx, P* dw, P* db, float* part, int* launches, cudaStream_t st) {
-    const GradShape g = grad_shape(rows, D);
+    GradShape g = grad_shape(rows, D);
     if (rows > 0 && g.warps == 0) {
         norm_grad_columns_kernel<T><<<dim3((D + 255) / 256, (unsigned)g.parts), 256, 0, st>>>(dy, ld_dy, x, ld_x, rows, D, mean, rstd,
                                                                                              part, g.ld_part);
@@ -399,15 +889,44 @@ cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int
         norm_grad_long_kernel<T, P><<<(unsigned)grid, 1024, 0, st>>>(dy, ld_dy, x, ld_x, rows, D, w, mean, rstd, dx, ld_dx);
         *launches += 2;
     } else if (rows > 0) {
-        constexpr int kVec = 16 / (int)sizeof(T) < kGradCols ? 16 / (int)sizeof(T) : kGradCols;
-        const int es = (int)sizeof(T);
-        const int vec = wide_elements({{x, ld_x, es}, {dy, ld_dy, es}, {dx, ld_dx, es}, {w, 0, (int)sizeof(P)}}, D, kVec);
-        if (vec == kVec)
-            norm_grad_kernel<T, P, kVec><<<g.blocks, g.threads, 0, st>>>(dy, ld_dy, x, ld_x, rows, D, w, mean, rstd, dx, ld_dx,
-                                                                        part, g.ld_part, g.warps);
-        else
-            norm_grad_kernel<T, P, 1><<<g.blocks, g.threads, 0, st>>>(dy, ld_dy, x, ld_x, rows, D, w, mean, rstd, dx, ld_dx,
-                                                                     part, g.ld_part, g.warps);
+        const int es = (int)sizeof(T), cols = D * es / 16;
+        const int vec = wide_elements({{x, ld_x, es}, {dy, ld_dy, es}, {dx, ld_dx, es}}, D, 16 / es);
+        const int slot = (D * es / 16 + 2) * 16;  // of a row that starts anywhere
+        auto go = [&](auto r_, auto lanes_, auto e_, auto s_) {
+            constexpr int R = decltype(r_)::value, LANES = decltype(lanes_)::value, E = decltype(e_)::value, S = decltype(s_)::value;
+            const auto kernel = norm_grad_rows_kernel<T, P, R, LANES, E, S>;
+            const int groups = g.threads / 32 / g.warps * (32 / LANES);
+            const size_t bytes = E == 0 ? (size_t)S * R * 2 * kGradCols * es * g.threads : (size_t)S * groups * R * 2 * slot + (size_t)g.warps * 32 * kGradCols * es;  // room past the last row
+            const cudaError_t e = allow_smem(kernel, bytes);
+            if (e != cudaSuccess) return e;
+            const int64_t need = (rows + groups * R - 1) / (groups * R);
+            if (need < g.parts) g.parts = need;
+            kernel<<<(unsigned)g.parts, g.threads, bytes, st>>>(dy, ld_dy, x, ld_x, rows, D, w, mean, rstd, dx, ld_dx, part, g.ld_part,
+                                                              g.warps, slot);
+            return cudaGetLastError();
+        };
+        const std::integral_constant<int, 0> i0;
+        const std::integral_constant<int, 1> i1;
+        const std::integral_constant<int, 2> i2;
+        const std::integral_constant<int, 3> i3;
+        const std::integral_constant<int, 4> i4;
+        const std::integral_constant<int, 32> all;
+        // four rows at a time where three stages of them fit into shared memory, else two
+        auto ragged = [&](auto e_) {
+            const size_t stage = (size_t)(g.threads / 32 / g.warps) * 4 * 2 * slot;
+            return 3 * stage <= 200 * 1024 ? go(i4, all, e_, i3) : go(i2, all, e_, i3);
+        };
+        cudaError_t e;
+        if (vec * es == 16) {
+            if (cols * (16 / es) <= 8 * kGradCols) e = go(i4, std::integral_constant<int, 8>{}, i0, i3);
+            else if (cols * (16 / es) <= 16 * kGradCols) e = go(i4, std::integral_constant<int, 16>{}, i0, i3);
+            else e = g.threads * es > 1024 ? go(i2, all, i0, i3) : go(i4, all, i0, i3);
+        } else if constexpr (sizeof(T) == 2) {
+            e = vec >= 2 ? ragged(i2) : ragged(i1);
+        } else {
+            e = ragged(i1);
+        }
+        if (e != cudaSuccess) return e;
         *launches += 1;
     }
     if (dw || db) {

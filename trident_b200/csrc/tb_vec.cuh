@@ -95,6 +95,45 @@ struct Pack {
     }
 };
 
+// Packed pairs of floats: one instruction for two operations.
+__device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
+
+// The 16 bytes at p as pairs of floats (4 of float32, 8 of a 16-bit type), and back.
+template <class T> constexpr int kPairs16 = 8 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& raw, float2* f) {
+    if constexpr (sizeof(T) == 4) {
+        f[0] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+        f[1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+    } else {
+        f[0] = unpack2<T>(raw.x);
+        f[1] = unpack2<T>(raw.y);
+        f[2] = unpack2<T>(raw.z);
+        f[3] = unpack2<T>(raw.w);
+    }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack16(const float2* f) {
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+    else
+        return make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y), pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y));
+}
+
+// 16 bytes from global to shared memory without a register, in groups that are waited for by count.
+__device__ __forceinline__ void copy16_async(void* smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem) : "memory");
+}
+// The same, or 16 bytes of zeros where !on (p is then not read, but is an address all the same).
+__device__ __forceinline__ void copy16_async_or_zero(void* smem, const void* p, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(p),
+                 "r"(on ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // N floats to or from memory of type T, in accesses of at most 16 bytes.
 template <class T, int N>
 __device__ __forceinline__ void load_n(const T* p, float* f) {
