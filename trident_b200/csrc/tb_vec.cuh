@@ -120,6 +120,20 @@ __device__ __forceinline__ uint4 pack16(const float2* f) {
         return make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y), pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y));
 }
 
+// sqrt(x) to a few units in the last place; values below 2^-126 count as 0.
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 1 / x to a unit in the last place for 2^-126 <= x <= 2^126; infinite below.
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // 16 bytes from global to shared memory without a register, in groups that are waited for by count.
 __device__ __forceinline__ void copy16_async(void* smem, const void* gmem) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(gmem) : "memory");
