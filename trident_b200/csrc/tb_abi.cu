@@ -55,6 +55,24 @@ namespace tb {
 static_assert(QI_LEN == TRIDENT_QINFO_LEN, "qinfo layout");
 
 int record_error(int code, const char* msg) { return fail(code, "%s", msg); }
+cudaError_t side_stream(SideStream** out) {
+    static thread_local SideStream per_dev[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) dev = 0;
+    SideStream& ss = per_dev[dev];
+    if (!ss.s) {
+        if ((e = cudaStreamCreateWithFlags(&ss.s, cudaStreamNonBlocking)) != cudaSuccess) return e;
+        if ((e = cudaEventCreateWithFlags(&ss.fork, cudaEventDisableTiming)) != cudaSuccess) return e;
+        if ((e = cudaEventCreateWithFlags(&ss.join, cudaEventDisableTiming)) != cudaSuccess) return e;
+        if ((e = cudaEventCreateWithFlags(&ss.fork2, cudaEventDisableTiming)) != cudaSuccess) return e;
+        if ((e = cudaEventCreateWithFlags(&ss.join2, cudaEventDisableTiming)) != cudaSuccess) return e;
+    }
+    *out = &ss;
+    return cudaSuccess;
+}
+
 void count_launches(int n) { g_launches += n; }
 int cuda_status(cudaError_t e, const char* where) { return e == cudaSuccess ? TRIDENT_OK : cuda_fail(e, where); }
 
@@ -236,32 +254,9 @@ struct Marker {
     }
 };
 
-// A second stream (and its fork/join events) per calling thread and device. The float64 rotation
-// runs there: the coarse GEMM, the probe selection and the pair lists need only the queries and
-// their norms, so the rotation overlaps all of them and is joined before the seed kernel.
-struct SideStream {
-    cudaStream_t s = nullptr;
-    cudaEvent_t fork = nullptr, join = nullptr;    // around the rotation
-    cudaEvent_t fork2 = nullptr, join2 = nullptr;  // around the pair lists and work items
-};
-
-static cudaError_t side_stream(SideStream** out) {
-    static thread_local SideStream per_dev[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) dev = 0;
-    SideStream& ss = per_dev[dev];
-    if (!ss.s) {
-        if ((e = cudaStreamCreateWithFlags(&ss.s, cudaStreamNonBlocking)) != cudaSuccess) return e;
-        if ((e = cudaEventCreateWithFlags(&ss.fork, cudaEventDisableTiming)) != cudaSuccess) return e;
-        if ((e = cudaEventCreateWithFlags(&ss.join, cudaEventDisableTiming)) != cudaSuccess) return e;
-        if ((e = cudaEventCreateWithFlags(&ss.fork2, cudaEventDisableTiming)) != cudaSuccess) return e;
-        if ((e = cudaEventCreateWithFlags(&ss.join2, cudaEventDisableTiming)) != cudaSuccess) return e;
-    }
-    *out = &ss;
-    return cudaSuccess;
-}
+// The float64 rotation runs on the side stream: the coarse GEMM, the probe selection and the pair lists
+// need only the queries and their norms, so the rotation overlaps all of them and is joined before the seed
+// kernel.
 
 // Stage 1 of a search: rotation, coarse GEMM and exact probe selection for B queries, into ws.
 static int stage_coarse(const trident_index* idx, const float* xq, int32_t B, int32_t nprobe, const Workspace& ws,

@@ -180,19 +180,24 @@ __global__ void __launch_bounds__(256) grad_direct_kernel(const T* __restrict__ 
 }
 
 // ---- gradient: stable radix sort of (id, position)
+//
+// Two launches a pass of up to 9 bits: the counts of each block's keys, then the keys to their places. A block
+// finds its places by adding up the counts of all blocks itself (at most kMaxTiles rows of 2 KB), which takes
+// the time of a few loads in flight and spares a launch.
 
-constexpr int kSortThreads = 512;
+constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxBins = 512;              // 9 bits a pass: two passes sort ids below 2^18
-constexpr int kSubTile = kSortThreads * 4;
+constexpr int kSortKeys = 4;               // keys of a thread in a turn
+constexpr int kSubTile = kSortThreads * kSortKeys;
 constexpr int kMaxTiles = 256;             // blocks of a pass; each reads the counts of all
 
 struct SortPass {
     const void* ids;       // pass 0
     int id64;
     int64_t V;
-    const int32_t* keys;   // later passes
-    const int32_t* pos;
+    const int2* in;        // later passes: (key, position)
+    int2* out;
     int32_t* n_valid;
     int64_t count;
     int64_t tile;          // positions of a block, a multiple of kSubTile
@@ -202,104 +207,125 @@ struct SortPass {
 // counts[block][digit] of the block's valid keys.
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass s, int32_t* __restrict__ counts, int32_t* status) {
     __shared__ int32_t hist[kMaxBins];
-    hist[threadIdx.x] = 0;
+    if (threadIdx.x < kMaxBins) hist[threadIdx.x] = 0;
     __syncthreads();
     const int64_t n = s.first ? s.count : (int64_t)*s.n_valid;
     const int64_t lo = (int64_t)blockIdx.x * s.tile, hi = min(n, lo + s.tile);
     const int mask = (1 << s.bits) - 1;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
-        const int32_t key = s.first ? valid_row(load_id(s.ids, s.id64, i), s.V, status) : s.keys[i];
-        if (key >= 0) atomicAdd(&hist[(key >> s.shift) & mask], 1);
+    for (int64_t sub = lo; sub < hi; sub += kSubTile) {
+        int32_t key[kSortKeys];
+#pragma unroll
+        for (int k = 0; k < kSortKeys; ++k) {
+            const int64_t i = sub + k * kSortThreads + threadIdx.x;
+            key[k] = -1;
+            if (i < hi) key[k] = s.first ? valid_row(load_id(s.ids, s.id64, i), s.V, status) : s.in[i].x;
+        }
+#pragma unroll
+        for (int k = 0; k < kSortKeys; ++k)
+            if (key[k] >= 0) atomicAdd(&hist[(key[k] >> s.shift) & mask], 1);
     }
     __syncthreads();
     if (threadIdx.x <= mask) counts[(int64_t)blockIdx.x * kMaxBins + threadIdx.x] = hist[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, const int32_t* __restrict__ counts, int tiles,
-                                                                    int32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out) {
-    __shared__ int32_t warp_hist[kSortWarps][kMaxBins];
+__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, const int32_t* __restrict__ counts, int tiles) {
+    extern __shared__ int32_t warp_hist[];  // [kSortWarps][kMaxBins]
     __shared__ int32_t offset[kMaxBins];
-    __shared__ int32_t scan[kSortWarps];
+    __shared__ int32_t halves[2][2][kMaxBins];
+    __shared__ int32_t scan[kMaxBins / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int mask = (1 << s.bits) - 1;
-    // where this block's keys of digit `tid` go: after all smaller digits, and this digit's in earlier blocks
-    int total = 0, before = 0;
-    if (tid <= mask) {
-#pragma unroll 8
-        for (int b = 0; b < tiles; ++b) {
-            const int c = counts[(int64_t)b * kMaxBins + tid];
-            total += c;
-            if (b < (int)blockIdx.x) before += c;
+    const int mask = (1 << s.bits) - 1, digit_of_thread = tid & (kMaxBins - 1), half = tid / kMaxBins;
+    // the first turn's keys are on their way meanwhile
+    int2 item[kSortKeys];
+    const int64_t most = s.count;  // (the later passes' arrays are as long; what is past n is not used)
+    const int64_t lo = (int64_t)blockIdx.x * s.tile;
+    auto load = [&](int64_t sub) {
+#pragma unroll
+        for (int k = 0; k < kSortKeys; ++k) {  // a warp's keys of a turn are consecutive
+            const int64_t i = sub + warp * (32 * kSortKeys) + k * 32 + lane;
+            item[k] = make_int2(-1, (int)i);
+            if (i < most) {
+                if (s.first) item[k].x = valid_row(load_id(s.ids, s.id64, i), s.V, nullptr);
+                else item[k] = s.in[i];
+            }
         }
+    };
+    load(lo);
+    // where this block's keys of a digit go: after all smaller digits, and this digit's in earlier blocks
+    {
+        int total = 0, before = 0;
+        if (digit_of_thread <= mask) {
+            const int b1 = half ? tiles : tiles / 2;
+#pragma unroll 16
+            for (int b = half ? tiles / 2 : 0; b < b1; ++b) {
+                const int c = counts[(int64_t)b * kMaxBins + digit_of_thread];
+                total += c;
+                if (b < (int)blockIdx.x) before += c;
+            }
+        }
+        halves[half][0][digit_of_thread] = total;
+        halves[half][1][digit_of_thread] = before;
     }
-    int incl = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int base = incl - total;
-    int all = 0;
+    int total = 0, incl = 0;
+    if (tid < kMaxBins) {
+        total = halves[0][0][tid] + halves[1][0][tid];
+        incl = total;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) scan[warp] = incl;
+    }
+    __syncthreads();
+    int all = 0, base = incl - total;
+#pragma unroll
+    for (int w = 0; w < kMaxBins / 32; ++w) {
         if (w < warp) base += scan[w];
         all += scan[w];
     }
-    offset[tid] = base + before;
+    if (tid < kMaxBins) offset[tid] = base + halves[0][1][tid] + halves[1][1][tid];
     if (s.first && blockIdx.x == 0 && tid == 0) *s.n_valid = all;
-    const int64_t n = s.first ? s.count : (int64_t)all;
-    const int64_t lo = (int64_t)blockIdx.x * s.tile, hi = min(n, lo + s.tile);
+    const int64_t n = s.first ? s.count : (int64_t)all, hi = min(n, lo + s.tile);
+    int32_t* mine = warp_hist + warp * kMaxBins;
     for (int64_t sub = lo; sub < hi; sub += kSubTile) {
-        for (int i = lane; i <= mask; i += 32) warp_hist[warp][i] = 0;
+        if (sub > lo) load(sub);
+        for (int i = lane; i <= mask; i += 32) mine[i] = 0;
         __syncwarp();
-        int32_t key[4], pos[4], rank[4];
+        int32_t rank[kSortKeys];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // a warp's 128 positions are consecutive
-            const int64_t i = sub + warp * 128 + k * 32 + lane;
-            key[k] = -1;
-            if (i < hi) {
-                key[k] = s.first ? valid_row(load_id(s.ids, s.id64, i), s.V, nullptr) : s.keys[i];
-                pos[k] = s.first ? (int32_t)i : s.pos[i];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int digit = (key[k] >> s.shift) & mask;
-            const unsigned valid = __ballot_sync(0xffffffffu, key[k] >= 0);
-            unsigned same = valid;  // lanes with this lane's digit
+        for (int k = 0; k < kSortKeys; ++k) {
+            if (sub + warp * (32 * kSortKeys) + k * 32 + lane >= hi) item[k].x = -1;
+            const int digit = (item[k].x >> s.shift) & mask;
+            unsigned same = __ballot_sync(0xffffffffu, item[k].x >= 0);  // lanes with this lane's digit
             for (int b = 0; b < s.bits; ++b) {
                 const unsigned set = __ballot_sync(0xffffffffu, (digit >> b) & 1);
                 same &= ((digit >> b) & 1) ? set : ~set;
             }
             const unsigned lower = same & ((1u << lane) - 1);
             int prior = 0;
-            if (key[k] >= 0) prior = warp_hist[warp][digit];
+            if (item[k].x >= 0) prior = mine[digit];
             __syncwarp();
-            if (key[k] >= 0 && lower == 0) warp_hist[warp][digit] = prior + __popc(same);
+            if (item[k].x >= 0 && lower == 0) mine[digit] = prior + __popc(same);
             __syncwarp();
             rank[k] = prior + __popc(lower);
         }
         __syncthreads();
         if (tid <= mask) {
             int at = offset[tid];
-#pragma unroll
+#pragma unroll 8
             for (int w = 0; w < kSortWarps; ++w) {
-                const int c = warp_hist[w][tid];
-                warp_hist[w][tid] = at;
+                const int c = warp_hist[w * kMaxBins + tid];
+                warp_hist[w * kMaxBins + tid] = at;
                 at += c;
             }
             offset[tid] = at;
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (key[k] < 0) continue;
-            const int dst = warp_hist[warp][(key[k] >> s.shift) & mask] + rank[k];
-            keys_out[dst] = key[k];
-            pos_out[dst] = pos[k];
-        }
+        for (int k = 0; k < kSortKeys; ++k)
+            if (item[k].x >= 0) s.out[mine[(item[k].x >> s.shift) & mask] + rank[k]] = item[k];
         __syncthreads();
     }
 }
@@ -309,88 +335,128 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, 
 constexpr int kPiece = 32;
 
 struct RunArgs {
-    const int32_t* keys;
-    const int32_t* pos;
+    const int2* items;   // (key, position), sorted, in whole pieces
     const int32_t* n_valid;
     float* part;         // [pieces][2][ld_part]: a run from the piece before, a run into the next
     int64_t ld_part;
     int64_t ld, ld_out;
+    int64_t count;       // ids, valid or not
     int cols;            // wide columns (D / VEC)
     int spans;           // ceil(cols / 32)
     float scale;
     int accumulate;
 };
 
+// *p += f without waiting for what was there. Each element is added to once in a call, so that no order of
+// the adds can change it.
+template <int N>
+__device__ __forceinline__ void add_at(float* p, const float* f) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + i), "f"(f[i]), "f"(f[i + 1]), "f"(f[i + 2]), "f"(f[i + 3]) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p + i), "f"(f[i]) : "memory");
+    }
+}
+
 template <class O, int VEC>
 __device__ __forceinline__ void finish_row(const RunArgs& a, O* out, int32_t key, int v, float* acc) {
     O* o = out + (int64_t)key * a.ld_out + (int64_t)v * VEC;
-    if (a.accumulate) {
+    if (sizeof(O) == 2 && a.accumulate) {
         float old[VEC];
         load_n<O, VEC>(o, old);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = fmaf(acc[i], a.scale, old[i]);
-    } else {
+        store_n<O, VEC>(o, acc);
+        return;
+    }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+    for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+    if constexpr (sizeof(O) == 4) {
+        if (a.accumulate) return add_at<VEC>(o, acc);
     }
     store_n<O, VEC>(o, acc);
 }
 
-template <class T, class O, int VEC>
+// LANES lanes sum one piece over one span of columns. Eight rows are loaded together, and where a 16-bit table
+// is added to (ACC), what it holds at the runs that end among them.
+template <class T, class O, int VEC, int LANES, bool ACC>
 __global__ void __launch_bounds__(256) run_sum_kernel(RunArgs a, const T* __restrict__ grad, O* __restrict__ out) {
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    constexpr int BATCH = 8;
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int64_t piece = unit / a.spans;
-    const int v = (int)(unit % a.spans) * 32 + lane;
+    const int v = (int)(unit - piece * a.spans) * LANES + lane;
     const int n = *a.n_valid;
     const int64_t first = piece * kPiece;
-    if (first >= n) return;
+    if (first >= n || v >= a.cols) return;
     const int m = (int)min((int64_t)kPiece, n - first);
-    const int32_t key = lane < m ? a.keys[first + lane] : -1;
-    const int32_t pos = lane < m ? a.pos[first + lane] : 0;
-    const int32_t prev = first > 0 ? a.keys[first - 1] : -1;
-    const int32_t next = first + m < n ? a.keys[first + m] : -1;
-    const bool on = v < a.cols;
+    const int32_t prev = first > 0 ? a.items[first - 1].x : -1;
+    const int32_t next = first + m < n ? a.items[first + m].x : -1;
     const T* col = grad + (int64_t)v * VEC;
     float acc[VEC] = {};
-    int start = 0;
-    for (int j0 = 0; j0 < m; j0 += 8) {
-        Pack<T, VEC> p[8];
+    bool from_before = false;
+    auto to_slot = [&](int which) { store_n<float, VEC>(a.part + (piece * 2 + which) * a.ld_part + (int64_t)v * VEC, acc); };
+    for (int j0 = 0; j0 < m; j0 += BATCH) {
+        int32_t key[BATCH + 1], pos[BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int32_t r = __shfl_sync(0xffffffffu, pos, j0 + k);
-            if (on && j0 + k < m) p[k] = Pack<T, VEC>::load_stream(col + (int64_t)r * a.ld);
+        for (int k = 0; k < BATCH; k += 2) {
+            const int4 two = *reinterpret_cast<const int4*>(a.items + first + j0 + k);
+            key[k] = two.x;
+            pos[k] = two.y;
+            key[k + 1] = two.z;
+            pos[k + 1] = two.w;
         }
+        key[BATCH] = j0 + BATCH < m ? a.items[first + j0 + BATCH].x : next;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int j = j0 + k;
-            const int32_t kj = __shfl_sync(0xffffffffu, key, j);
-            const int32_t after = __shfl_sync(0xffffffffu, key, (j + 1) & 31);
-            if (j >= m) continue;
-            if (on) {
-                float f[VEC];
-                p[k].get(f);
+        for (int k = 0; k < BATCH; ++k)
+            if (j0 + k >= m) key[k] = next;  // -1 there: past the last id
+        Pack<T, VEC> p[BATCH];
+        constexpr bool OLD = ACC && sizeof(O) == 2;
+        Pack<O, sizeof(O) == 2 ? VEC : 1> old[OLD ? BATCH : 1];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[i] += f[i];
-            }
-            const bool last = j + 1 == m;
-            if (last || after != kj) {
-                const bool from_before = start == 0 && prev == kj;
-                const bool into_next = last && next == kj;
-                if (on) {
-                    if (from_before || into_next) {
-                        float* slot = a.part + (piece * 2 + (from_before ? 0 : 1)) * a.ld_part + (int64_t)v * VEC;
-                        store_n<float, VEC>(slot, acc);
+        for (int k = 0; k < BATCH; ++k)
+            if (j0 + k < m) p[k] = Pack<T, VEC>::load_stream(col + (int64_t)pos[k] * a.ld);
+        if constexpr (OLD) {
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k)
+                if (j0 + k < m && key[k + 1] != key[k]) old[k] = Pack<O, VEC>::load(out + (int64_t)key[k] * a.ld_out + (int64_t)v * VEC);
+        }
+        if (j0 == 0) from_before = prev == key[0];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (j0 + k >= m) break;
+            float f[VEC];
+            p[k].get(f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] += f[i];
+            if (key[k + 1] != key[k]) {  // the run's end
+                if (from_before) {
+                    to_slot(0);
+                    from_before = false;
+                } else {
+                    O* o = out + (int64_t)key[k] * a.ld_out + (int64_t)v * VEC;
+                    if constexpr (OLD) {
+                        float was[VEC];
+                        old[k].get(was);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(acc[i], a.scale, was[i]);
+                        store_n<O, VEC>(o, acc);
                     } else {
-                        finish_row<O, VEC>(a, out, kj, v, acc);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+                        if constexpr (ACC) add_at<VEC>(o, acc);
+                        else store_n<O, VEC>(o, acc);
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-                start = j + 1;
             }
         }
     }
+    if (m == kPiece && next == a.items[first + kPiece - 1].x) to_slot(from_before ? 0 : 1);  // into the next piece
 }
 
 constexpr int kJoinAlone = 16;  // partial sums that one warp adds by itself
@@ -407,9 +473,8 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
     const int v = (int)(blockIdx.x % a.spans) * 32 + lane;
     const bool on = v < a.cols;
     const int64_t piece = group * 8 + warp;
-    const int n = *a.n_valid;
     auto add = [&](float* acc, int64_t lo, int64_t hi) {  // slot 0 of pieces [lo, hi)
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t q = lo; q < hi; ++q) {
             float f[VEC];
             load_n<float, VEC>(a.part + q * 2 * a.ld_part + (int64_t)v * VEC, f);
@@ -419,17 +484,28 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
     };
     bool is_long = false;
     const int64_t end = (piece + 1) * kPiece;
-    if (end < n) {
-        const int32_t key = a.keys[end - 1];
-        const bool crosses = a.keys[end] == key;
-        const bool begins = a.keys[end - kPiece] != key || piece == 0 || a.keys[end - kPiece - 1] != key;
-        if (crosses && begins) {
-            int64_t lo = end, hi = n;  // the run's end: the first position of a larger key
-            while (lo < hi) {
-                const int64_t mid = (lo + hi) >> 1;
-                if (a.keys[mid] == key) lo = mid + 1; else hi = mid;
+    if (end < a.count) {
+        // everything that the first decisions need, at once (n bounds what of it is meant)
+        const int n = *a.n_valid;
+        const int32_t key = a.items[end - 1].x, after = a.items[end].x, head = a.items[end - kPiece].x;
+        const int32_t before = piece > 0 ? a.items[end - kPiece - 1].x : -1;
+        // piece q's first key, and whether the run of `key` reaches its end
+        auto probe = [&](int64_t q, int32_t& first_key) {
+            first_key = q * kPiece < a.count ? a.items[q * kPiece].x : -1;
+            return (q + 1) * kPiece <= n && a.items[(q + 1) * kPiece - 1].x == key;
+        };
+        int32_t first_key;
+        int64_t known = piece;  // the run reaches this piece's end
+        unsigned miss = ~__ballot_sync(0xffffffffu, probe(known + 1 + lane, first_key));
+        if (end < n && after == key && (head != key || before != key)) {
+            if (miss == 0) {  // in steps of 32 pieces, then the last 32
+                known += 32;
+                while ((miss = ~__ballot_sync(0xffffffffu, probe(known + 32 * (lane + 1), first_key))) == 0) known += 1024;
+                known += 32 * (__ffs(miss) - 1);
+                miss = ~__ballot_sync(0xffffffffu, probe(known + 1 + lane, first_key));
             }
-            const int64_t last = (lo - 1) / kPiece;
+            int64_t last = known + __ffs(miss);
+            if (last * kPiece >= n || __shfl_sync(0xffffffffu, first_key, __ffs(miss) - 1) != key) --last;  // ended before
             if (last - piece < kJoinAlone) {
                 if (on) {
                     float acc[VEC];
@@ -474,8 +550,7 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
 struct GradWorkspace {
     int32_t* n_valid;
     int32_t* counts;     // [kMaxTiles][kMaxBins]
-    int32_t* keys[2];
-    int32_t* pos[2];
+    int2* items[2];
     float* part;
 };
 
@@ -492,10 +567,10 @@ size_t carve_grad(int64_t T, int D, void* base, GradWorkspace* ws) {
     GradWorkspace w;
     w.n_valid = (int32_t*)take(256);
     if (T > kDirectIds) {
+        const size_t pieces = (size_t)((T + kPiece - 1) / kPiece);
         w.counts = (int32_t*)take((size_t)kMaxTiles * kMaxBins * 4);
-        for (int i = 0; i < 2; ++i) w.keys[i] = (int32_t*)take((size_t)T * 4);
-        for (int i = 0; i < 2; ++i) w.pos[i] = (int32_t*)take((size_t)T * 4);
-        w.part = (float*)take((size_t)((T + kPiece - 1) / kPiece) * 2 * part_stride(D) * 4);
+        for (int i = 0; i < 2; ++i) w.items[i] = (int2*)take(pieces * kPiece * sizeof(int2));
+        w.part = (float*)take(pieces * 2 * part_stride(D) * 4);
     }
     if (ws) *ws = w;
     return off;
@@ -506,14 +581,24 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
                        int accumulate, O* out, int64_t ld_out, void* workspace, int32_t* status, int* launches,
                        cudaStream_t st) {
     cudaError_t e;
-    if (!accumulate) {
-        e = ld_out == D ? cudaMemsetAsync(out, 0, (size_t)V * D * sizeof(O), st)
-                        : cudaMemset2DAsync(out, ld_out * sizeof(O), 0, (size_t)D * sizeof(O), V, st);
-        if (e != cudaSuccess) return e;
-    }
-    if (count == 0) return cudaSuccess;
     constexpr int kMax = 16 / (int)sizeof(T);
     int vec = wide_elements({{grad, ld, (int)sizeof(T)}, {out, ld_out, (int)sizeof(O)}}, D, kMax);
+    SideStream* side = nullptr;  // zeros are written beside the sort
+    if (!accumulate && V > 0) {
+        const int64_t row_bytes = (int64_t)D * sizeof(O);
+        cudaStream_t zs = st;
+        if (count > kDirectIds) {
+            if ((e = side_stream(&side)) != cudaSuccess) return e;
+            if ((e = cudaEventRecord(side->fork, st)) != cudaSuccess) return e;
+            if ((e = cudaStreamWaitEvent(side->s, side->fork, 0)) != cudaSuccess) return e;
+            zs = side->s;
+        }
+        e = ld_out == D ? cudaMemsetAsync(out, 0, (size_t)V * row_bytes, zs)
+                        : cudaMemset2DAsync(out, ld_out * sizeof(O), 0, (size_t)row_bytes, V, zs);
+        if (e != cudaSuccess) return e;
+        if (side && (e = cudaEventRecord(side->join, side->s)) != cudaSuccess) return e;
+    }
+    if (count == 0) return cudaSuccess;
     if (count <= kDirectIds) {
         with_vec<kMax>(vec, [&](auto v) {
             constexpr int VEC = decltype(v)::value;
@@ -527,27 +612,30 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     carve_grad(count, D, workspace, &ws);
     int bits = 1;
     while (bits < 31 && ((int64_t)1 << bits) < V) ++bits;
-    const int passes = (bits + 8) / 9;
+    const int passes = (bits + 8) / 9, pass_bits = (bits + passes - 1) / passes;
     SortPass s;
     s.ids = ids;
     s.id64 = id64;
     s.V = V;
     s.n_valid = ws.n_valid;
     s.count = count;
-    s.bits = (bits + passes - 1) / passes;
+    s.bits = pass_bits;
     s.tile = ((count + kMaxTiles - 1) / kMaxTiles + kSubTile - 1) / kSubTile * kSubTile;
     const int tiles = (int)((count + s.tile - 1) / s.tile);
+    constexpr int kSmem = kSortWarps * kMaxBins * 4;
+    if ((e = allow_smem(sort_scatter_kernel, kSmem)) != cudaSuccess) return e;
     for (int p = 0; p < passes; ++p) {
         s.first = p == 0;
         s.shift = p * s.bits;
-        s.keys = ws.keys[(p + 1) & 1];
-        s.pos = ws.pos[(p + 1) & 1];
+        s.in = ws.items[(p + 1) & 1];
+        s.out = ws.items[p & 1];
         sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, status);
-        sort_scatter_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, tiles, ws.keys[p & 1], ws.pos[p & 1]);
+        sort_scatter_kernel<<<tiles, kSortThreads, kSmem, st>>>(s, ws.counts, tiles);
     }
+    if (side && (e = cudaStreamWaitEvent(st, side->join, 0)) != cudaSuccess) return e;
     RunArgs a;
-    a.keys = ws.keys[(passes - 1) & 1];
-    a.pos = ws.pos[(passes - 1) & 1];
+    a.items = ws.items[(passes - 1) & 1];
+    a.count = count;
     a.n_valid = ws.n_valid;
     a.part = ws.part;
     a.ld_part = part_stride(D);
@@ -555,16 +643,26 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     a.ld_out = ld_out;
     a.scale = scale;
     a.accumulate = accumulate;
-    while (vec > 1 && D / vec < 32) vec /= 2;  // a narrow row over all lanes of a warp
     a.cols = D / vec;
-    a.spans = (a.cols + 31) / 32;
     const int64_t pieces = (count + kPiece - 1) / kPiece;
-    const int64_t grid = (pieces * a.spans + 7) / 8, join_grid = (pieces + 7) / 8 * a.spans;
+    const int lanes = a.cols > 16 ? 32 : a.cols > 8 ? 16 : 8;
+    a.spans = (a.cols + lanes - 1) / lanes;
+    const int join_spans = (a.cols + 31) / 32;
+    const int64_t grid = (pieces * a.spans * lanes + 255) / 256, join_grid = (pieces + 7) / 8 * join_spans;
     if (grid > 0x7fffffff || join_grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     with_vec<kMax>(vec, [&](auto v) {
         constexpr int VEC = decltype(v)::value;
-        run_sum_kernel<T, O, VEC><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
-        run_join_kernel<O, VEC><<<(unsigned)join_grid, 256, 0, st>>>(a, out);
+        auto go = [&](auto l) {
+            constexpr int LANES = decltype(l)::value;
+            if (accumulate) run_sum_kernel<T, O, VEC, LANES, true><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
+            else run_sum_kernel<T, O, VEC, LANES, false><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
+        };
+        if (lanes == 32) go(std::integral_constant<int, 32>{});
+        else if (lanes == 16) go(std::integral_constant<int, 16>{});
+        else go(std::integral_constant<int, 8>{});
+        RunArgs j = a;
+        j.spans = join_spans;
+        run_join_kernel<O, VEC><<<(unsigned)join_grid, 256, 0, st>>>(j, out);
     });
     *launches += 2 * passes + 2;
     return cudaGetLastError();

@@ -128,6 +128,15 @@ cudaError_t launch_merge_shards(const float* d_in, const int64_t* i_in, int R, i
 
 int num_sms();
 
+// A second stream (and its fork/join events) per calling thread and device, for work that runs beside the
+// caller's stream (tb_abi.cu).
+struct SideStream {
+    cudaStream_t s = nullptr;
+    cudaEvent_t fork = nullptr, join = nullptr;    // around the rotation, or a gradient's zeros
+    cudaEvent_t fork2 = nullptr, join2 = nullptr;  // around the pair lists and work items
+};
+cudaError_t side_stream(SideStream** out);
+
 // Store `msg` as the calling thread's last error (trident_last_error) and return `code`.
 int record_error(int code, const char* msg);
 
