@@ -565,8 +565,8 @@ size_t carve_grad(int64_t T, int D, void* base, GradWorkspace* ws) {
         return r;
     };
     GradWorkspace w;
-    w.n_valid = (int32_t*)take(256);
     if (T > kDirectIds) {
+        w.n_valid = (int32_t*)take(256);
         const size_t pieces = (size_t)((T + kPiece - 1) / kPiece);
         w.counts = (int32_t*)take((size_t)kMaxTiles * kMaxBins * 4);
         for (int i = 0; i < 2; ++i) w.items[i] = (int2*)take(pieces * kPiece * sizeof(int2));
@@ -623,7 +623,7 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     s.tile = ((count + kMaxTiles - 1) / kMaxTiles + kSubTile - 1) / kSubTile * kSubTile;
     const int tiles = (int)((count + s.tile - 1) / s.tile);
     constexpr int kSmem = kSortWarps * kMaxBins * 4;
-    if ((e = allow_smem(sort_scatter_kernel, kSmem)) != cudaSuccess) return e;
+    if ((e = allow_smem<sort_scatter_kernel>(kSmem)) != cudaSuccess) return e;
     for (int p = 0; p < passes; ++p) {
         s.first = p == 0;
         s.shift = p * s.bits;

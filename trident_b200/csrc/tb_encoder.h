@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -57,12 +58,20 @@ void with_vec(int vec, F&& f) {
     f(std::integral_constant<int, 1>{});
 }
 
-// Lets a kernel have `bytes` of dynamic shared memory on the current device (48 KB in all, the kernel's own
-// static memory among them, need no leave).
-template <class K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
+// Lets KERNEL have `bytes` of dynamic shared memory on the current device (48 KB in all, its own static
+// memory among them, need no leave). What it was last given on a device is remembered.
+template <auto KERNEL>
+cudaError_t allow_smem(size_t bytes) {
     if (bytes <= 40 * 1024) return cudaSuccess;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    static std::atomic<size_t> given[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool known = dev >= 0 && dev < 64;
+    if (known && given[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && known) given[dev].store(bytes, std::memory_order_relaxed);
+    return e;
 }
 
 cudaError_t launch_embed_lookup(const void* table, int dtype, int64_t V, int D, int64_t ld, const void* ids, int id64,

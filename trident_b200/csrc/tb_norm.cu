@@ -442,7 +442,7 @@ cudaError_t norm_typed(const T* x, int64_t rows, int D, int64_t ld_x, const P* w
         auto stream = [&](auto k, auto l) {
             constexpr int NV = decltype(k)::value, LANES = decltype(l)::value;
             const size_t bytes = (size_t)kRowWarps * kStages * kRowsAtOnce<NV> * NV * 32 * 16 + (size_t)D * 8;
-            const cudaError_t e = allow_smem(norm_rows_kernel<T, P, NV, LANES>, bytes);
+            const cudaError_t e = allow_smem<norm_rows_kernel<T, P, NV, LANES>>(bytes);
             if (e != cudaSuccess) return e;
             const int per_sm = bytes <= 112 * 1024 ? 2 : 1;  // of 227 KB, 1 KB a block the system's
             norm_rows_kernel<T, P, NV, LANES><<<num_sms() * per_sm, 32 * kRowWarps, bytes, st>>>(x, rows, D, ld_x, w, b, eps, y,
@@ -464,7 +464,7 @@ cudaError_t norm_typed(const T* x, int64_t rows, int D, int64_t ld_x, const P* w
         auto stream = [&](auto e_, auto k, auto s_) {
             constexpr int E = decltype(e_)::value, NV = decltype(k)::value, S = decltype(s_)::value;
             const size_t bytes = (size_t)(kRowWarps / warps) * S * slot + (size_t)D * 8;
-            const cudaError_t e = allow_smem(norm_ragged_kernel<T, P, E, NV, S>, bytes);
+            const cudaError_t e = allow_smem<norm_ragged_kernel<T, P, E, NV, S>>(bytes);
             if (e != cudaSuccess) return e;
             const int per_sm = bytes <= 112 * 1024 ? 2 : 1;
             norm_ragged_kernel<T, P, E, NV, S><<<num_sms() * per_sm, 32 * kRowWarps, bytes, st>>>(x, rows, D, ld_x, w, b, eps, y, ld_y,
@@ -894,10 +894,10 @@ cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int
         const int slot = (D * es / 16 + 2) * 16;  // of a row that starts anywhere
         auto go = [&](auto r_, auto lanes_, auto e_, auto s_) {
             constexpr int R = decltype(r_)::value, LANES = decltype(lanes_)::value, E = decltype(e_)::value, S = decltype(s_)::value;
-            const auto kernel = norm_grad_rows_kernel<T, P, R, LANES, E, S>;
+            constexpr auto kernel = norm_grad_rows_kernel<T, P, R, LANES, E, S>;
             const int groups = g.threads / 32 / g.warps * (32 / LANES);
             const size_t bytes = E == 0 ? (size_t)S * R * 2 * kGradCols * es * g.threads : (size_t)S * groups * R * 2 * slot + (size_t)g.warps * 32 * kGradCols * es;  // room past the last row
-            const cudaError_t e = allow_smem(kernel, bytes);
+            const cudaError_t e = allow_smem<kernel>(bytes);
             if (e != cudaSuccess) return e;
             const int64_t need = (rows + groups * R - 1) / (groups * R);
             if (need < g.parts) g.parts = need;

@@ -11,6 +11,7 @@ same inputs give the same bits. Inputs may have a row stride; one without unit s
 transposed or broadcast tensor) is copied first.
 """
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -27,12 +28,6 @@ def _dtype(t, name: str) -> int:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     return code
-
-
-def _same_device(dev, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
 def _rows(t, D: int):
@@ -52,19 +47,31 @@ def _out_rows(t, D: int, name: str) -> int:
     raise ValueError(f"{name} must be contiguous, or 2-D with unit stride in its last dim")
 
 
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+# The current stream's handle by device index. torch's own accessor builds a Stream object, 2 us of a call
+# that takes 7; the raw one is used where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(dev, fn, *args) -> None:
     """fn(*args, current stream) with dev as the current device."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(dev))
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _stream(dev))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, device_index: int, *sizes) -> int:
+    """Workspace bytes of an operator (a function of its sizes and the device alone)."""
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device_index):
+        _lib.check(getattr(_lib.lib(), name)(*sizes, ctypes.byref(need)))
+    return need.value
 
 
 def _p(t):
@@ -103,7 +110,7 @@ def embedding_lookup(table, ids, scale: float = 1.0, out=None, status=None):
     _status(status, dev)
     shape = (*ids.shape, D)
     if out is None:
-        out, ld_out = torch.empty(shape, dtype=table.dtype, device=dev), D
+        out, ld_out = table.new_empty(shape), D
     else:
         if out.shape != shape or out.dtype != table.dtype or out.device != dev:
             raise ValueError(f"out must be a {table.dtype} tensor of shape {shape} on {dev}")
@@ -131,17 +138,16 @@ def embedding_grad(grad_out, ids, num_rows: int, scale: float = 1.0, out=None, a
     if out is None:
         if accumulate:
             raise ValueError("accumulate=True needs out")
-        out, ld_out = torch.empty((V, D), dtype=dtype or grad_out.dtype, device=dev), D
+        out, ld_out = grad_out.new_empty((V, D), dtype=dtype), D
     else:
         if out.shape != (V, D) or out.device != dev or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out must be a {dtype or ''} tensor of shape {(V, D)} on {dev}")
         ld_out = _out_rows(out, D, "out")
-    out_code, L, T = _dtype(out, "out"), _lib.lib(), ids.numel()
-    need = ctypes.c_size_t(0)
-    _lib.check(L.trident_embed_grad_workspace_size(T, V, D, ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    _call(dev, L.trident_embed_grad, grad_out.data_ptr(), code, ld, ids.data_ptr(), bits, T, V, D, scale,
-          int(accumulate), out.data_ptr(), out_code, ld_out, ws.data_ptr(), need.value, _p(status))
+    out_code, T = _dtype(out, "out"), ids.numel()
+    need = _workspace_bytes("trident_embed_grad_workspace_size", dev.index, T, V, D)
+    ws = grad_out.new_empty(need, dtype=torch.uint8) if need else None
+    _call(dev, _lib.lib().trident_embed_grad, grad_out.data_ptr(), code, ld, ids.data_ptr(), bits, T, V, D, scale,
+          int(accumulate), out.data_ptr(), out_code, ld_out, _p(ws), need, _p(status))
     return out
 
 
@@ -171,7 +177,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bo
     shape, rows = x.shape, x.numel() // D
     if out is None:
         x, ld = _rows(x, D)
-        out, ld_out = torch.empty(shape, dtype=x.dtype, device=dev), D
+        out, ld_out = x.new_empty(shape), D
     else:
         if out.shape != shape or out.dtype != x.dtype or out.device != dev:
             raise ValueError(f"out must be a {x.dtype} tensor of shape {tuple(shape)} on {dev}")
@@ -179,7 +185,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bo
         x, ld = _rows(x, D)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, *shape[:-1]), dtype=torch.float32, device=dev)
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     _call(dev, _lib.lib().trident_layer_norm, x.data_ptr(), code, rows, D, ld, _p(weight), _p(bias), pcode, eps,
           out.data_ptr(), ld_out, _p(mean), _p(rstd))
     return (out, mean, rstd) if stats else out
@@ -204,20 +211,19 @@ def layer_norm_grad(grad_out, x, weight, mean, rstd, out=None, param_grads: bool
     pcode = code if weight is None else _dtype(weight, "weight")
     shape, rows = x.shape, x.numel() // D
     if out is None:
-        out, ld_out = torch.empty(shape, dtype=x.dtype, device=dev), D
+        out, ld_out = x.new_empty(shape), D
     else:
         if out.shape != shape or out.dtype != x.dtype or out.device != dev:
             raise ValueError(f"out must be a {x.dtype} tensor of shape {tuple(shape)} on {dev}")
         ld_out = _out_rows(out, D, "out")
     x, ld_x = _rows(x, D)
     grad_out, ld_dy = _rows(grad_out, D)
-    L, need = _lib.lib(), ctypes.c_size_t(0)
-    _lib.check(L.trident_layer_norm_grad_workspace_size(rows, D, ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    need = _workspace_bytes("trident_layer_norm_grad_workspace_size", dev.index, rows, D)
+    ws = x.new_empty(need, dtype=torch.uint8)
     dw = db = None
     if param_grads:
-        pdtype = x.dtype if weight is None else weight.dtype
-        dw, db = torch.empty((2, D), dtype=pdtype, device=dev)
-    _call(dev, L.trident_layer_norm_grad, grad_out.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, rows, D, _p(weight),
-          pcode, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), ld_out, _p(dw), _p(db), ws.data_ptr(), need.value)
+        dw = x.new_empty(D) if weight is None else torch.empty_like(weight)
+        db = torch.empty_like(dw)
+    _call(dev, _lib.lib().trident_layer_norm_grad, grad_out.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, rows, D, _p(weight),
+          pcode, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), ld_out, _p(dw), _p(db), ws.data_ptr(), need)
     return out, dw, db

@@ -62,7 +62,8 @@ class AdamW:
                     d.v, d.m_scale, d.v_scale = (s[k].data_ptr() for k in ("exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale"))
                 if self.master and dtype != torch.float32:
                     d.master = s["master"].data_ptr()
-            self._groups.append((dtype, at, desc))
+            self._groups.append((dtype, [(i, d, self.params[i].shape, d.n) for i, d in zip(at, desc)], desc))
+        self._config = _lib.AdamWConfig(state_bits=state_bits)
 
     def _states(self, given) -> dict:
         P = self.params
@@ -102,38 +103,36 @@ class AdamW:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != self.dev):
             raise ValueError(f"grad_scale must be one float32 on {self.dev}")
-        t = self.step_count + 1
-        c = _lib.AdamWConfig()
-        c.state_bits, c.step = self.state_bits, t
-        c.lr = self.lr if lr is None else float(lr)
-        c.beta1, c.beta2 = self.betas
-        c.eps, c.weight_decay = self.eps, self.weight_decay
-        c.grad_scale = None if grad_scale is None else grad_scale.data_ptr()
         keep = []  # copies of gradients that were not contiguous
         calls = []
-        for dtype, at, desc in self._groups:
+        index = self.dev.index
+        for dtype, tensors, desc in self._groups:
             gdtype = None
-            for d, i in zip(desc, at):
-                g, p = grads[i], self.params[i]
+            for i, d, shape, n in tensors:
+                g = grads[i]
                 if g is None:
                     d.n = 0
                     continue
-                if g.shape != p.shape or g.device != self.dev:
-                    raise ValueError(f"gradient {i} must have its parameter's shape and device")
-                if gdtype is None:
+                if g.dtype is not gdtype:
+                    if gdtype is not None:
+                        raise ValueError(f"gradient {i} is {g.dtype}, others of {dtype} parameters are {gdtype}")
                     gdtype = g.dtype
                     if gdtype != dtype and gdtype != torch.float32:
                         raise ValueError(f"gradient {i} must be {dtype} or float32, not {gdtype}")
-                elif g.dtype != gdtype:
-                    raise ValueError(f"gradient {i} is {g.dtype}, others of {dtype} parameters are {gdtype}")
+                if g.shape != shape or g.get_device() != index:
+                    raise ValueError(f"gradient {i} must have its parameter's shape and device")
                 if not g.is_contiguous():
                     g = g.contiguous()
                     keep.append(g)
-                d.grad, d.n = g.data_ptr(), p.numel()
+                d.grad, d.n = g.data_ptr(), n
             if gdtype is not None:
-                calls.append((dtype, gdtype, desc))
-        for k, (dtype, gdtype, desc) in enumerate(calls):
-            c.param_dtype, c.grad_dtype = _DTYPES[dtype], _DTYPES[gdtype]
+                calls.append((_DTYPES[dtype], _DTYPES[gdtype], desc))
+        t, c = self.step_count + 1, self._config
+        c.step, c.lr = t, self.lr if lr is None else lr
+        c.beta1, c.beta2 = self.betas
+        c.eps, c.weight_decay = self.eps, self.weight_decay
+        c.grad_scale = None if grad_scale is None else grad_scale.data_ptr()
+        for k, (c.param_dtype, c.grad_dtype, desc) in enumerate(calls):
             c.rounding_seed = (self.seed + t * _SEED_STEP + k) & 0xFFFFFFFF
             _call(self.dev, _lib.lib().trident_adamw_step, desc, len(desc), ctypes.byref(c))
         self.step_count = t
