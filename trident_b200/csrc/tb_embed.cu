@@ -8,6 +8,8 @@
 // span of columns. A run inside a piece is written at once; a run that crosses a border leaves one partial
 // sum for each piece, and a second kernel adds those in order. No float is added by an atomic, so the sums
 // have one order, which the ids alone fix.
+#include <cooperative_groups.h>
+
 #include "tb_encoder.h"
 #include "tb_vec.cuh"
 
@@ -229,12 +231,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass s, in
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, const int32_t* __restrict__ counts, int tiles) {
-    extern __shared__ int32_t warp_hist[];  // [kSortWarps][kMaxBins]
-    __shared__ int32_t offset[kMaxBins];
-    __shared__ int32_t halves[2][2][kMaxBins];
-    __shared__ int32_t scan[kMaxBins / 32];
+    extern __shared__ __align__(16) int32_t warp_hist[];  // [kSortWarps][kMaxBins], then the turn's items in order
+    __shared__ int32_t offset[kMaxBins];   // where the block's next key of a digit goes
+    __shared__ int32_t start[kMaxBins];    // ... and its first of this turn in `sorted`
+    __shared__ __align__(16) int32_t sums[2][kSortThreads * 4 / kMaxBins][kMaxBins];
+    __shared__ int32_t scan[2][kMaxBins / 32];
+    int2* sorted = reinterpret_cast<int2*>(warp_hist + kSortWarps * kMaxBins);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int mask = (1 << s.bits) - 1, digit_of_thread = tid & (kMaxBins - 1), half = tid / kMaxBins;
+    const int mask = (1 << s.bits) - 1;
     // the first turn's keys are on their way meanwhile
     int2 item[kSortKeys];
     const int64_t most = s.count;  // (the later passes' arrays are as long; what is past n is not used)
@@ -251,41 +255,56 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, 
         }
     };
     load(lo);
-    // where this block's keys of a digit go: after all smaller digits, and this digit's in earlier blocks
+    // where this block's keys of a digit go: after all smaller digits, and this digit's in earlier blocks.
+    // Four digits a thread; the rows of counts are shared by kParts sets of threads.
+    constexpr int kQuads = kMaxBins / 4, kParts = kSortThreads / kQuads;
     {
-        int total = 0, before = 0;
-        if (digit_of_thread <= mask) {
-            const int b1 = half ? tiles : tiles / 2;
-#pragma unroll 16
-            for (int b = half ? tiles / 2 : 0; b < b1; ++b) {
-                const int c = counts[(int64_t)b * kMaxBins + digit_of_thread];
-                total += c;
-                if (b < (int)blockIdx.x) before += c;
+        int4 total = make_int4(0, 0, 0, 0), before = total;
+        const int quad = tid & (kQuads - 1), part = tid / kQuads;
+        if (quad * 4 <= mask) {
+#pragma unroll 8
+            for (int b = part; b < tiles; b += kParts) {
+                const int4 c = *reinterpret_cast<const int4*>(counts + (int64_t)b * kMaxBins + quad * 4);
+                total.x += c.x; total.y += c.y; total.z += c.z; total.w += c.w;
+                if (b < (int)blockIdx.x) { before.x += c.x; before.y += c.y; before.z += c.z; before.w += c.w; }
             }
         }
-        halves[half][0][digit_of_thread] = total;
-        halves[half][1][digit_of_thread] = before;
+        *reinterpret_cast<int4*>(&sums[0][part][quad * 4]) = total;
+        *reinterpret_cast<int4*>(&sums[1][part][quad * 4]) = before;
     }
     __syncthreads();
-    int total = 0, incl = 0;
-    if (tid < kMaxBins) {
-        total = halves[0][0][tid] + halves[1][0][tid];
-        incl = total;
+    // exclusive sum over the digits of one value a digit, by the first kMaxBins threads; `all`: their sum
+    auto scan_bins = [&](int value, int which, int& all) {
+        int incl = value;
+        if (tid < kMaxBins) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (lane == 31) scan[which][warp] = incl;
         }
-        if (lane == 31) scan[warp] = incl;
-    }
-    __syncthreads();
-    int all = 0, base = incl - total;
+        __syncthreads();
+        int base = incl - value;
+        all = 0;
 #pragma unroll
-    for (int w = 0; w < kMaxBins / 32; ++w) {
-        if (w < warp) base += scan[w];
-        all += scan[w];
+        for (int w = 0; w < kMaxBins / 32; ++w) {
+            const int c = scan[which][w];
+            if (w < warp) base += c;
+            all += c;
+        }
+        return base;
+    };
+    int total = 0, before = 0, all;
+    if (tid <= mask) {
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+            total += sums[0][q][tid];
+            before += sums[1][q][tid];
+        }
     }
-    if (tid < kMaxBins) offset[tid] = base + halves[0][1][tid] + halves[1][1][tid];
+    const int base = scan_bins(total, 0, all);
+    if (tid < kMaxBins) offset[tid] = base + before;
     if (s.first && blockIdx.x == 0 && tid == 0) *s.n_valid = all;
     const int64_t n = s.first ? s.count : (int64_t)all, hi = min(n, lo + s.tile);
     int32_t* mine = warp_hist + warp * kMaxBins;
@@ -312,22 +331,158 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, 
             rank[k] = prior + __popc(lower);
         }
         __syncthreads();
+        int count = 0, turn;
         if (tid <= mask) {
-            int at = offset[tid];
 #pragma unroll 8
             for (int w = 0; w < kSortWarps; ++w) {
                 const int c = warp_hist[w * kMaxBins + tid];
-                warp_hist[w * kMaxBins + tid] = at;
-                at += c;
+                warp_hist[w * kMaxBins + tid] = count;
+                count += c;
             }
-            offset[tid] = at;
+        }
+        const int first = scan_bins(count, 1, turn);
+        if (tid < kMaxBins) start[tid] = first;
+        __syncthreads();
+        // in order in shared memory first: the keys of a digit then leave together
+#pragma unroll
+        for (int k = 0; k < kSortKeys; ++k) {
+            const int digit = (item[k].x >> s.shift) & mask;
+            if (item[k].x >= 0) sorted[start[digit] + mine[digit] + rank[k]] = item[k];
         }
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kSortKeys; ++k)
-            if (item[k].x >= 0) s.out[mine[(item[k].x >> s.shift) & mask] + rank[k]] = item[k];
+        for (int i = tid; i < turn; i += kSortThreads) {
+            const int2 it = sorted[i];
+            const int digit = (it.x >> s.shift) & mask;
+            s.out[offset[digit] + i - start[digit]] = it;
+        }
+        __syncthreads();
+        if (tid <= mask) offset[tid] += count;
         __syncthreads();
     }
+}
+
+// The whole sort in one launch, for up to kClusterIds ids: a cluster of kClusterBlocks thread blocks, whose
+// barriers stand where the launches above part. Each warp owns a run of positions: it counts its digits, the
+// counts are added up over the block's warps and then over the cluster's blocks (read from their shared
+// memory), and the warp goes over its keys again in order. More ids than that are written out faster by more
+// SMs than a cluster has: 32,000 ids below 65,536 take %CL32% us here and %ML32% us in separate launches,
+// 131,072 ids %CL131% and %ML131% us.
+constexpr int kClusterBlocks = 16;
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int64_t kClusterIds = 131072;
+constexpr int kClusterSmem = (kClusterWarps + 2) * kMaxBins * 4;
+
+struct ClusterSort {
+    const void* ids;
+    int id64;
+    int64_t V;
+    int count, bits, passes;
+    int2* items[2];
+    int32_t *n_valid, *status;
+};
+
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(ClusterSort s) {
+    extern __shared__ int32_t sh[];
+    __shared__ int32_t scan[kClusterWarps];
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int32_t* mine = sh + warp * kMaxBins;            // this warp's counts, then where its next key of a digit goes
+    int32_t* total = sh + kClusterWarps * kMaxBins;  // the block's counts
+    int32_t* offset = total + kMaxBins;
+    const int rank = (int)cluster.block_rank();
+    const int bins = 1 << s.bits;
+    const int seg = ((s.count + kClusterBlocks * kClusterWarps - 1) / (kClusterBlocks * kClusterWarps) + 31) / 32 * 32;
+    const int lo = (rank * kClusterWarps + warp) * seg;
+    int n = s.count;
+    for (int p = 0; p < s.passes; ++p) {
+        const int shift = p * s.bits;
+        const int2* in = s.items[(p + 1) & 1];
+        int2* out = s.items[p & 1];
+        const int hi = min(n, lo + seg);
+        auto load = [&](int i0, int2* item, int32_t* status) {  // kSortKeys rounds of 32 at a time
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k) {
+                const int i = i0 + k * 32 + lane;
+                item[k] = make_int2(-1, i);
+                if (i < hi) {
+                    if (p == 0) item[k].x = valid_row(load_id(s.ids, s.id64, i), s.V, status);
+                    else item[k] = __ldcg(in + i);
+                }
+            }
+        };
+        for (int i = lane; i < bins; i += 32) mine[i] = 0;
+        __syncwarp();
+        int2 item[kSortKeys];
+        for (int i0 = lo; i0 < hi; i0 += 32 * kSortKeys) {
+            load(i0, item, s.status);
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k)
+                if (item[k].x >= 0) atomicAdd(&mine[(item[k].x >> shift) & (bins - 1)], 1);
+        }
+        __syncthreads();
+        if (tid < bins) {
+            int sum = 0;
+#pragma unroll 8
+            for (int w = 0; w < kClusterWarps; ++w) {
+                const int c = sh[w * kMaxBins + tid];
+                sh[w * kMaxBins + tid] = sum;
+                sum += c;
+            }
+            total[tid] = sum;
+        }
+        cluster.sync();
+        int all = 0, before = 0;
+        if (tid < bins) {
+#pragma unroll
+            for (int r = 0; r < kClusterBlocks; ++r) {
+                const int c = cluster.map_shared_rank(total, r)[tid];
+                all += c;
+                if (r < rank) before += c;
+            }
+        }
+        int incl = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        int base = incl - all;
+        n = 0;  // from the first pass on, the valid ids
+#pragma unroll
+        for (int w = 0; w < kMaxBins / 32; ++w) {
+            const int c = scan[w];
+            if (w < warp) base += c;
+            n += c;
+        }
+        if (tid < bins) offset[tid] = base + before;
+        __syncthreads();
+        const bool once = lo + 32 * kSortKeys >= hi;  // the keys are still in registers
+        for (int i0 = lo; i0 < hi; i0 += 32 * kSortKeys) {
+            if (!once) load(i0, item, nullptr);
+#pragma unroll
+            for (int k = 0; k < kSortKeys; ++k) {
+                if (i0 + k * 32 >= hi) break;
+                const int digit = (item[k].x >> shift) & (bins - 1);
+                unsigned same = __ballot_sync(0xffffffffu, item[k].x >= 0);  // lanes with this lane's digit
+                for (int b = 0; b < s.bits; ++b) {
+                    const unsigned set = __ballot_sync(0xffffffffu, (digit >> b) & 1);
+                    same &= ((digit >> b) & 1) ? set : ~set;
+                }
+                const unsigned lower = same & ((1u << lane) - 1);
+                int prior = 0;
+                if (item[k].x >= 0) prior = mine[digit];
+                __syncwarp();
+                if (item[k].x >= 0 && lower == 0) mine[digit] = prior + __popc(same);
+                __syncwarp();
+                if (item[k].x >= 0) out[offset[digit] + prior + __popc(lower)] = item[k];
+            }
+        }
+        cluster.sync();
+    }
+    if (rank == 0 && tid == 0) *s.n_valid = n;
 }
 
 // ---- gradient: sums of the sorted runs
@@ -462,24 +617,37 @@ __global__ void __launch_bounds__(256) run_sum_kernel(RunArgs a, const T* __rest
 constexpr int kJoinAlone = 16;  // partial sums that one warp adds by itself
 
 // Adds the partial sums of each run that crosses pieces: slot 1 of its first piece, then slot 0 of the
-// others, in order. One warp per (piece, span); a long run is shared by the block's 8 warps.
-template <class O, int VEC>
+// others. One warp per (piece, span of LANES wide columns); its 32 / LANES sets of lanes take turns of the
+// partial sums, and a long run is shared by the block's 8 warps.
+template <class O, int VEC, int LANES>
 __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict__ out) {
     __shared__ int64_t long_first[8], long_last[8];
     __shared__ int32_t long_key[8];
-    __shared__ __align__(16) float sums[8][32 * VEC];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ __align__(16) float sums[8][LANES * VEC];
+    constexpr int SETS = 32 / LANES;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, set = lane / LANES;
     const int64_t group = blockIdx.x / a.spans;
-    const int v = (int)(blockIdx.x % a.spans) * 32 + lane;
+    const int v = (int)(blockIdx.x % a.spans) * LANES + (lane & (LANES - 1));
     const bool on = v < a.cols;
     const int64_t piece = group * 8 + warp;
-    auto add = [&](float* acc, int64_t lo, int64_t hi) {  // slot 0 of pieces [lo, hi)
-#pragma unroll 8
-        for (int64_t q = lo; q < hi; ++q) {
-            float f[VEC];
-            load_n<float, VEC>(a.part + q * 2 * a.ld_part + (int64_t)v * VEC, f);
+    // the sum of slot 0 of pieces [lo, hi), and of slot 1 of piece `head` if it is one (>= 0), in every lane
+    auto add = [&](float* acc, int64_t head, int64_t lo, int64_t hi) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] += f[i];
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+        if (on) {
+            if (head >= 0 && set == 0) load_n<float, VEC>(a.part + (head * 2 + 1) * a.ld_part + (int64_t)v * VEC, acc);
+#pragma unroll 8
+            for (int64_t q = lo + (head >= 0 ? (set + SETS - 1) % SETS : set); q < hi; q += SETS) {
+                float f[VEC];
+                load_n<float, VEC>(a.part + q * 2 * a.ld_part + (int64_t)v * VEC, f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[i] += f[i];
+            }
+        }
+#pragma unroll
+        for (int o = LANES; o < 32; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
         }
     };
     bool is_long = false;
@@ -507,12 +675,9 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
             int64_t last = known + __ffs(miss);
             if (last * kPiece >= n || __shfl_sync(0xffffffffu, first_key, __ffs(miss) - 1) != key) --last;  // ended before
             if (last - piece < kJoinAlone) {
-                if (on) {
-                    float acc[VEC];
-                    load_n<float, VEC>(a.part + (piece * 2 + 1) * a.ld_part + (int64_t)v * VEC, acc);
-                    add(acc, piece + 1, last + 1);
-                    finish_row<O, VEC>(a, out, key, v, acc);
-                }
+                float acc[VEC];
+                add(acc, piece, piece + 1, last + 1);
+                if (on && set == 0) finish_row<O, VEC>(a, out, key, v, acc);
             } else {
                 is_long = true;
                 if (lane == 0) {
@@ -528,15 +693,14 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
     for (int r = 0; r < 8; ++r) {
         if (long_key[r] < 0) continue;
         const int64_t lo = long_first[r] + 1, m = long_last[r] + 1 - lo;
-        float acc[VEC] = {};
-        if (on) {
-            if (warp == 0) load_n<float, VEC>(a.part + (long_first[r] * 2 + 1) * a.ld_part + (int64_t)v * VEC, acc);
-            add(acc, lo + m * warp / 8, lo + m * (warp + 1) / 8);
-        }
+        float acc[VEC];
+        add(acc, warp == 0 ? long_first[r] : -1, lo + m * warp / 8, lo + m * (warp + 1) / 8);
+        if (set == 0) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sums[warp][lane * VEC + i] = acc[i];
+            for (int i = 0; i < VEC; ++i) sums[warp][lane * VEC + i] = acc[i];
+        }
         __syncthreads();
-        if (warp == 0 && on) {
+        if (warp == 0 && set == 0 && on) {
 #pragma unroll
             for (int w = 1; w < 8; ++w)
 #pragma unroll
@@ -576,6 +740,27 @@ size_t carve_grad(int64_t T, int D, void* base, GradWorkspace* ws) {
     return off;
 }
 
+cudaError_t launch_cluster_sort(const ClusterSort& s, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = allow_smem<sort_cluster_kernel>(kClusterSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kClusterBlocks);
+    cfg.blockDim = dim3(kClusterThreads);
+    cfg.dynamicSmemBytes = kClusterSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kClusterBlocks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, sort_cluster_kernel, s);
+}
+
+// Zeros that take longer than a fork and a join of streams cost are written beside the sort.
+constexpr int64_t kSideZeros = 16 << 20;
+
 template <class T, class O>
 cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int64_t count, int64_t V, int D, float scale,
                        int accumulate, O* out, int64_t ld_out, void* workspace, int32_t* status, int* launches,
@@ -587,7 +772,7 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     if (!accumulate && V > 0) {
         const int64_t row_bytes = (int64_t)D * sizeof(O);
         cudaStream_t zs = st;
-        if (count > kDirectIds) {
+        if (count > kDirectIds && V * row_bytes >= kSideZeros) {
             if ((e = side_stream(&side)) != cudaSuccess) return e;
             if ((e = cudaEventRecord(side->fork, st)) != cudaSuccess) return e;
             if ((e = cudaStreamWaitEvent(side->s, side->fork, 0)) != cudaSuccess) return e;
@@ -613,24 +798,40 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     int bits = 1;
     while (bits < 31 && ((int64_t)1 << bits) < V) ++bits;
     const int passes = (bits + 8) / 9, pass_bits = (bits + passes - 1) / passes;
-    SortPass s;
-    s.ids = ids;
-    s.id64 = id64;
-    s.V = V;
-    s.n_valid = ws.n_valid;
-    s.count = count;
-    s.bits = pass_bits;
-    s.tile = ((count + kMaxTiles - 1) / kMaxTiles + kSubTile - 1) / kSubTile * kSubTile;
-    const int tiles = (int)((count + s.tile - 1) / s.tile);
-    constexpr int kSmem = kSortWarps * kMaxBins * 4;
-    if ((e = allow_smem<sort_scatter_kernel>(kSmem)) != cudaSuccess) return e;
-    for (int p = 0; p < passes; ++p) {
-        s.first = p == 0;
-        s.shift = p * s.bits;
-        s.in = ws.items[(p + 1) & 1];
-        s.out = ws.items[p & 1];
-        sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, status);
-        sort_scatter_kernel<<<tiles, kSortThreads, kSmem, st>>>(s, ws.counts, tiles);
+    if (count <= kClusterIds) {
+        ClusterSort s;
+        s.ids = ids;
+        s.id64 = id64;
+        s.V = V;
+        s.count = (int)count;
+        s.bits = pass_bits;
+        s.passes = passes;
+        for (int i = 0; i < 2; ++i) s.items[i] = ws.items[i];
+        s.n_valid = ws.n_valid;
+        s.status = status;
+        if ((e = launch_cluster_sort(s, st)) != cudaSuccess) return e;
+        *launches += 1;
+    } else {
+        SortPass s;
+        s.ids = ids;
+        s.id64 = id64;
+        s.V = V;
+        s.n_valid = ws.n_valid;
+        s.count = count;
+        s.bits = pass_bits;
+        s.tile = ((count + kMaxTiles - 1) / kMaxTiles + kSubTile - 1) / kSubTile * kSubTile;
+        const int tiles = (int)((count + s.tile - 1) / s.tile);
+        constexpr int kSmem = kSortWarps * kMaxBins * 4 + kSubTile * (int)sizeof(int2);
+        if ((e = allow_smem<sort_scatter_kernel>(kSmem)) != cudaSuccess) return e;
+        for (int p = 0; p < passes; ++p) {
+            s.first = p == 0;
+            s.shift = p * s.bits;
+            s.in = ws.items[(p + 1) & 1];
+            s.out = ws.items[p & 1];
+            sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, status);
+            sort_scatter_kernel<<<tiles, kSortThreads, kSmem, st>>>(s, ws.counts, tiles);
+        }
+        *launches += 2 * passes;
     }
     if (side && (e = cudaStreamWaitEvent(st, side->join, 0)) != cudaSuccess) return e;
     RunArgs a;
@@ -647,8 +848,7 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     const int64_t pieces = (count + kPiece - 1) / kPiece;
     const int lanes = a.cols > 16 ? 32 : a.cols > 8 ? 16 : 8;
     a.spans = (a.cols + lanes - 1) / lanes;
-    const int join_spans = (a.cols + 31) / 32;
-    const int64_t grid = (pieces * a.spans * lanes + 255) / 256, join_grid = (pieces + 7) / 8 * join_spans;
+    const int64_t grid = (pieces * a.spans * lanes + 255) / 256, join_grid = (pieces + 7) / 8 * a.spans;
     if (grid > 0x7fffffff || join_grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     with_vec<kMax>(vec, [&](auto v) {
         constexpr int VEC = decltype(v)::value;
@@ -656,15 +856,13 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
             constexpr int LANES = decltype(l)::value;
             if (accumulate) run_sum_kernel<T, O, VEC, LANES, true><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
             else run_sum_kernel<T, O, VEC, LANES, false><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
+            run_join_kernel<O, VEC, LANES><<<(unsigned)join_grid, 256, 0, st>>>(a, out);
         };
         if (lanes == 32) go(std::integral_constant<int, 32>{});
         else if (lanes == 16) go(std::integral_constant<int, 16>{});
         else go(std::integral_constant<int, 8>{});
-        RunArgs j = a;
-        j.spans = join_spans;
-        run_join_kernel<O, VEC><<<(unsigned)join_grid, 256, 0, st>>>(j, out);
     });
-    *launches += 2 * passes + 2;
+    *launches += 2;
     return cudaGetLastError();
 }
 
