@@ -209,6 +209,7 @@ struct SortPass {
 // counts[block][digit] of the block's valid keys.
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass s, int32_t* __restrict__ counts, int32_t* status) {
     __shared__ int32_t hist[kMaxBins];
+    wait_for_previous();
     if (threadIdx.x < kMaxBins) hist[threadIdx.x] = 0;
     __syncthreads();
     const int64_t n = s.first ? s.count : (int64_t)*s.n_valid;
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortPass s, 
     __shared__ __align__(16) int32_t sums[2][kSortThreads * 4 / kMaxBins][kMaxBins];
     __shared__ int32_t scan[2][kMaxBins / 32];
     int2* sorted = reinterpret_cast<int2*>(warp_hist + kSortWarps * kMaxBins);
+    wait_for_previous();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int mask = (1 << s.bits) - 1;
     // the first turn's keys are on their way meanwhile
@@ -385,6 +387,7 @@ struct ClusterSort {
 __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(ClusterSort s) {
     extern __shared__ int32_t sh[];
     __shared__ int32_t scan[kClusterWarps];
+    wait_for_previous();
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int32_t* mine = sh + warp * kMaxBins;            // this warp's counts, then where its next key of a digit goes
@@ -540,6 +543,7 @@ __device__ __forceinline__ void finish_row(const RunArgs& a, O* out, int32_t key
 template <class T, class O, int VEC, int LANES, bool ACC>
 __global__ void __launch_bounds__(256) run_sum_kernel(RunArgs a, const T* __restrict__ grad, O* __restrict__ out) {
     constexpr int BATCH = 8;
+    wait_for_previous();
     const int lane = threadIdx.x & (LANES - 1);
     const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int64_t piece = unit / a.spans;
@@ -625,6 +629,7 @@ __global__ void __launch_bounds__(256) run_join_kernel(RunArgs a, O* __restrict_
     __shared__ int32_t long_key[8];
     __shared__ __align__(16) float sums[8][LANES * VEC];
     constexpr int SETS = 32 / LANES;
+    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, set = lane / LANES;
     const int64_t group = blockIdx.x / a.spans;
     const int v = (int)(blockIdx.x % a.spans) * LANES + (lane & (LANES - 1));
@@ -828,8 +833,9 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
             s.shift = p * s.bits;
             s.in = ws.items[(p + 1) & 1];
             s.out = ws.items[p & 1];
-            sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, status);
-            sort_scatter_kernel<<<tiles, kSortThreads, kSmem, st>>>(s, ws.counts, tiles);
+            if (p == 0) sort_count_kernel<<<tiles, kSortThreads, 0, st>>>(s, ws.counts, status);
+            else if ((e = launch_chained(sort_count_kernel, tiles, kSortThreads, 0, st, s, ws.counts, status)) != cudaSuccess) return e;
+            if ((e = launch_chained(sort_scatter_kernel, tiles, kSortThreads, kSmem, st, s, ws.counts, tiles)) != cudaSuccess) return e;
         }
         *launches += 2 * passes;
     }
@@ -854,16 +860,21 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
         constexpr int VEC = decltype(v)::value;
         auto go = [&](auto l) {
             constexpr int LANES = decltype(l)::value;
-            if (accumulate) run_sum_kernel<T, O, VEC, LANES, true><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
-            else run_sum_kernel<T, O, VEC, LANES, false><<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
-            run_join_kernel<O, VEC, LANES><<<(unsigned)join_grid, 256, 0, st>>>(a, out);
+            const auto sum = accumulate ? run_sum_kernel<T, O, VEC, LANES, true> : run_sum_kernel<T, O, VEC, LANES, false>;
+            if (side) {
+                sum<<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
+                e = cudaGetLastError();
+            } else {
+                e = launch_chained(sum, grid, 256, 0, st, a, grad, out);
+            }
+            if (e == cudaSuccess) e = launch_chained(run_join_kernel<O, VEC, LANES>, join_grid, 256, 0, st, a, out);
         };
         if (lanes == 32) go(std::integral_constant<int, 32>{});
         else if (lanes == 16) go(std::integral_constant<int, 16>{});
         else go(std::integral_constant<int, 8>{});
     });
     *launches += 2;
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace

@@ -74,6 +74,23 @@ cudaError_t allow_smem(size_t bytes) {
     return e;
 }
 
+// Launches a kernel that may come onto the GPU before the one before it on the stream has ended (it waits for
+// that end itself, wait_for_previous(), before it touches memory): the gap between two launches is hidden.
+template <class... P, class... A>
+cudaError_t launch_chained(void (*kernel)(P...), int64_t grid, int block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 cudaError_t launch_embed_lookup(const void* table, int dtype, int64_t V, int D, int64_t ld, const void* ids, int id64,
                                 int64_t count, float scale, void* out, int64_t ld_out, int32_t* status, cudaStream_t st);
 size_t embed_grad_workspace(int64_t T, int D);

@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(32 * kGradMaxWarps)
     constexpr int PER = 32 / LANES;
     extern __shared__ __align__(16) uint4 smem[];
     __shared__ __align__(16) float slots[2][kGradMaxWarps * PER][2 * R];
+    wait_for_previous();
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, sub = lane & (LANES - 1);
     const int in_row = warp % warps, warp_group = warp / warps;
     const int group = LANES < 32 ? tid / LANES : warp_group;
@@ -786,25 +787,27 @@ __global__ void __launch_bounds__(32 * kGradMaxWarps)
     }
 }
 
-// dw and db (blockIdx.y) of 32 columns a block: 32 lanes of partial rows each, added in order.
+// dw (the first half of the blocks) and db of 32 columns a block: 32 sets of partial rows each, added in order.
 template <class P>
 __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t ld_part,
                                                              int D, P* dw, P* db) {
     __shared__ float s[32][33];
-    P* out = blockIdx.y ? db : dw;
+    wait_for_previous();
+    const bool second = blockIdx.x >= gridDim.x / 2;
+    P* out = second ? db : dw;
     if (!out) return;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + tx;
+    const int c0 = (second ? blockIdx.x - gridDim.x / 2 : blockIdx.x) * 32, c = c0 + tx;
     float acc = 0.0f;
     if (c < D) {
-        const float* p = part + blockIdx.y * ld_part + c;
+        const float* p = part + (second ? ld_part : 0) + c;
 #pragma unroll 8
         for (int64_t q = ty; q < parts; q += 32) acc += p[q * 2 * ld_part];
     }
     s[ty][tx] = acc;
     __syncthreads();
     acc = warp_sum(s[tx][ty]);  // column ty of the block
-    const int cc = blockIdx.x * 32 + ty;
+    const int cc = c0 + ty;
     if (tx == 0 && cc < D) out[cc] = from_float<P>(acc);
 }
 
@@ -899,8 +902,10 @@ cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int
             const size_t bytes = E == 0 ? (size_t)S * R * 2 * kGradCols * es * g.threads : (size_t)S * groups * R * 2 * slot + (size_t)g.warps * 32 * kGradCols * es;  // room past the last row
             const cudaError_t e = allow_smem<kernel>(bytes);
             if (e != cudaSuccess) return e;
+            // no more blocks than are resident: each has its share of the rows from the start
+            const int64_t resident = (int64_t)num_sms() * (g.threads == 256 && bytes <= 108 * 1024 ? 2 : 1);
             const int64_t need = (rows + groups * R - 1) / (groups * R);
-            if (need < g.parts) g.parts = need;
+            g.parts = need < resident ? need : resident;
             kernel<<<(unsigned)g.parts, g.threads, bytes, st>>>(dy, ld_dy, x, ld_x, rows, D, w, mean, rstd, dx, ld_dx, part, g.ld_part,
                                                               g.warps, slot);
             return cudaGetLastError();
@@ -930,7 +935,9 @@ cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int
         *launches += 1;
     }
     if (dw || db) {
-        norm_grad_sum_kernel<P><<<dim3((D + 31) / 32, 2), 1024, 0, st>>>(part, rows > 0 ? g.parts : 0, g.ld_part, D, dw, db);
+        const cudaError_t e = launch_chained(norm_grad_sum_kernel<P>, (D + 31) / 32 * 2, 1024, 0, st, part, rows > 0 ? g.parts : 0,
+                                             g.ld_part, D, dw, db);
+        if (e != cudaSuccess) return e;
         *launches += 1;
     }
     return cudaGetLastError();

@@ -162,6 +162,13 @@ __device__ __forceinline__ void store_n(T* p, const float* f) {
     for (int i = 0; i < N; i += M) Pack<T, M>::of(f + i).store(p + i);
 }
 
+// For kernels of launch_chained: waits for the end of the kernel before (at once after any other launch), then
+// lets the one after come onto the GPU.
+__device__ __forceinline__ void wait_for_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -85,7 +85,7 @@ def _ids(ids, dev):
         bits = 32
     else:
         raise ValueError(f"ids must be int32 or int64, not {ids.dtype}")
-    if ids.device != dev:
+    if ids.get_device() != dev.index:
         raise ValueError(f"ids are on {ids.device}, not on {dev}")
     return (ids if ids.is_contiguous() else ids.contiguous()), bits
 
@@ -154,7 +154,7 @@ def embedding_grad(grad_out, ids, num_rows: int, scale: float = 1.0, out=None, a
 def _norm_param(t, name, D, x):
     if t is None:
         return
-    if t.shape != (D,) or not t.is_contiguous() or t.device != x.device:
+    if t.dim() != 1 or t.numel() != D or not t.is_contiguous() or t.get_device() != x.get_device():
         raise ValueError(f"{name} must be contiguous, of shape ({D},), on {x.device}")
 
 
