@@ -916,10 +916,11 @@ cudaError_t grad_typed(const T* dy, int64_t ld_dy, const T* x, int64_t ld_x, int
         const std::integral_constant<int, 3> i3;
         const std::integral_constant<int, 4> i4;
         const std::integral_constant<int, 32> all;
-        // four rows at a time where three stages of them fit into shared memory, else two
+        // four rows at a time where two blocks an SM have room for three stages of them, else two (50,000 x 1001
+        // float32: 145 us with four rows and one block, 123 us with two and two)
         auto ragged = [&](auto e_) {
             const size_t stage = (size_t)(g.threads / 32 / g.warps) * 4 * 2 * slot;
-            return 3 * stage <= 200 * 1024 ? go(i4, all, e_, i3) : go(i2, all, e_, i3);
+            return 3 * stage <= 104 * 1024 ? go(i4, all, e_, i3) : go(i2, all, e_, i3);
         };
         cudaError_t e;
         if (vec * es == 16) {
