@@ -154,6 +154,10 @@ GRAD_SHAPES = [
     (1025, 1, 16, "spread"), (2048, 512, 32, "skewed"), (2049, 513, 31, "skewed"), (4096, 2000, 1, "skewed"),
     (6145, 262_144, 8, "spread"), (5000, 300_000, 12, "skewed"), (20_011, 70, 128, "skewed"), (1300, 40, 960, "none"),
     (40_000, 3, 64, "same"), (33_333, 2, 9, "spread"), (3000, 1500, 1032, "skewed"),
+    # more ids than one cluster sorts, and more than fill the blocks of a pass once
+    (140_001, 3000, 8, "skewed"), (131_073, 70_000, 16, "spread"), (1_100_000, 300_000, 4, "skewed"), (200_000, 1, 8, "same"),
+    # zeros written beside the sort
+    (5000, 20_000, 500, "skewed"),
 ]
 
 
@@ -300,8 +304,15 @@ NORM_SHAPES = [(1, 1), (1, 8), (5, 7), (33, 96), (100, 128), (3, 960), (17, 961)
                (3, 2050), (2, 4096), (2, 4097), (3, 8192), (2, 8200), (1, 20_001), (2000, 72)]
 
 
+# as many rows as stay with resident warps: every number of columns a lane, several warps a row, rows that start
+# anywhere (at 4-byte places where D is even)
+MANY_ROWS = [(40_000, 24), (20_000, 64), (20_001, 128), (19_000, 200), (19_000, 500), (19_001, 960), (19_000, 1024), (10_000, 2048),
+             (5000, 4096), (2500, 8192), (5001, 33), (5000, 98), (5000, 201), (5000, 350), (5001, 1001), (5000, 1022), (2600, 2050),
+             (1300, 4099), (700, 8190)]
+
+
 @pytest.mark.parametrize("dtype,param", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float32")])
-@pytest.mark.parametrize("rows,D", NORM_SHAPES)
+@pytest.mark.parametrize("rows,D", NORM_SHAPES + MANY_ROWS)
 def test_layer_norm(dtype, param, rows, D):
     import torch
 
@@ -318,6 +329,41 @@ def test_layer_norm(dtype, param, rows, D):
     _close(tb.layer_norm(_strided(x, 1), w, b, stats=False), *_norm_reference(x, w, b, 1e-5, dtype)[0])
     inplace = x.clone()
     assert tb.layer_norm(inplace, w, b, out=inplace, stats=False) is inplace and torch.equal(inplace, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D,pad,skip", [(5000, 96, 8, 0), (5000, 100, 0, 1), (20_000, 64, 5, 3), (300, 97, 4, 1), (20_000, 960, 64, 0)])
+def test_layer_norm_of_a_window(dtype, rows, D, pad, skip):
+    """Rows inside wider rows, from a column on: strides and bases that allow wide loads and that do not. What lies
+    around the window is NaN, and stays."""
+    import torch
+
+    import trident_b200 as tb
+
+    wide = torch.full((rows + 1, D + pad + skip), float("nan"), dtype=_dt(dtype), device="cuda")
+    x = wide[:rows, skip:skip + D]
+    x.copy_(_randn((rows, D), dtype, 1, 1.5, 0.7))
+    w, b = _randn((D,), dtype, 2, 0.3, 1.0), _randn((D,), dtype, 3)
+    for got, (want, tol) in zip(tb.layer_norm(x, w, b), _norm_reference(x, w, b, 1e-5, dtype)):
+        _close(got, want, tol)
+    _, mean, rstd = tb.layer_norm(x)
+    dy = torch.full_like(wide, float("nan"))[:rows, skip:skip + D]
+    dy.copy_(_randn((rows, D), dtype, 4))
+    before = wide.clone()
+    out = wide[:rows, skip:skip + D]
+    y = torch.empty_like(wide)
+    y.fill_(7.0)
+    tb.layer_norm(x, w, b, out=y[:rows, skip:skip + D], stats=False)
+    _close(y[:rows, skip:skip + D], *_norm_reference(x, w, b, 1e-5, dtype)[0])
+    assert bool((y[rows:] == 7).all()) and bool((y[:, :skip] == 7).all()) and bool((y[:, skip + D:] == 7).all())
+    want = _norm_grad_reference(dy, x, w, mean, rstd, dtype, dtype)
+    got = tb.layer_norm_grad(dy, x, w, mean, rstd, out=y[:rows, skip:skip + D])
+    for g, (ref, tol) in zip(got, want):
+        _close(g, ref, tol)
+    assert bool((y[rows:] == 7).all()) and bool((y[:, :skip] == 7).all()) and bool((y[:, skip + D:] == 7).all())
+    assert torch.equal(wide.nan_to_num(9.0), before.nan_to_num(9.0)) and out.shape == x.shape
+    tb.layer_norm(x, w, b, out=x, stats=False)  # in place
+    assert torch.equal(torch.isnan(wide), torch.isnan(before))
 
 
 def test_layer_norm_values():
@@ -365,7 +411,7 @@ def _norm_grad_reference(dy, x, w, mean, rstd, dtype, param):
 
 
 @pytest.mark.parametrize("dtype,param", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float32")])
-@pytest.mark.parametrize("rows,D", NORM_SHAPES + [(6000, 96), (777, 1032), (130, 4100)])
+@pytest.mark.parametrize("rows,D", NORM_SHAPES + [(6000, 96), (777, 1032), (130, 4100), (9000, 64), (9000, 128), (3000, 98), (3000, 1001)])
 def test_layer_norm_gradient(dtype, param, rows, D):
     import torch
 

@@ -281,7 +281,7 @@ template <class P, class G, bool MASTER, bool BITS8>
 cudaError_t run(const trident_adamw_tensor* tensors, int count, Scalars s, int* launches, cudaStream_t st) {
     auto go = [&](auto cap, int lo, int n, uint32_t* blocks) {
         constexpr int CAP = decltype(cap)::value;
-        static thread_local Tensors<CAP> a;
+        Tensors<CAP> a;
         a.count = n;
         a.s = s;
         uint32_t at = 0, unit = 0;
