@@ -599,6 +599,14 @@ def run_ours(args, d: Dist):
     xs = perm = off = None
     check = None
     n_cpu = 0 if args.no_cpu_baseline else min(B, CPU_SAMPLE_CAP.get(cfg.name.split("_")[0], B))
+    cpu = None
+    if n_cpu:  # the reference's CPU path is timed only where its module is built
+        from oracle import ref_cpu
+
+        try:
+            ref_cpu.load()
+        except FileNotFoundError as e:
+            n_cpu, cpu = 0, {"unavailable": str(e)}
     if d.rank == 0:
         # host rows of every list that the checked queries and the CPU-baseline sample probe
         t0 = time.perf_counter()
@@ -718,7 +726,6 @@ def run_ours(args, d: Dist):
                             tensor=idx.stage_y_tensor(B * d.world, nprobe, K, args.ub_seed))
             if d.world > 1:
                 roof["scope"] = f"rank 0's scan: all {B * d.world} queries over rank 0's lists"
-        cpu = None
         if n_cpu:
             cpu = cpu_baseline(args, cfg, xq, c_np, xs, perm, off, n_cpu)
         ooc = ooc_acc
