@@ -67,7 +67,7 @@ class AdamW:
             # the descriptors' columns that a step writes, as one array each
             fields = np.frombuffer(desc, dtype=np.dtype(_lib.AdamWTensor))
             shapes = [self.params[i].shape for i in at]
-            self._groups.append((dtype, at, shapes, fields["n"].copy(), desc, fields["grad"], fields["n"]))
+            self._groups.append((dtype, at, shapes, fields["n"].copy(), desc, list(desc), fields["grad"], fields["n"]))
         self._config = _lib.AdamWConfig(state_bits=state_bits)
         self._partial = False  # the last step left some tensors out
 
@@ -111,7 +111,7 @@ class AdamW:
             raise ValueError(f"grad_scale must be one float32 on {self.dev}")
         keep, calls = [], []  # keep: copies of gradients that were not contiguous
         partial = False
-        for dtype, at, shapes, sizes, desc, grad_field, n_field in self._groups:
+        for dtype, at, shapes, sizes, desc, each, grad_field, n_field in self._groups:
             mine = grads if len(at) == len(grads) else [grads[i] for i in at]
             given = [g for g in mine if g is not None]
             if not given:
@@ -128,7 +128,11 @@ class AdamW:
                 given = [g.contiguous() for g in given]
                 keep.append(given)
             if all_given:
-                grad_field[:] = list(map(torch.Tensor.data_ptr, given))
+                if len(each) <= 12:  # an array's assignment costs as much as twelve fields'
+                    for d, g in zip(each, given):
+                        d.grad = g.data_ptr()
+                else:
+                    grad_field[:] = list(map(torch.Tensor.data_ptr, given))
                 if self._partial:
                     n_field[:] = sizes
             else:
