@@ -304,8 +304,9 @@ cudaError_t run(const trident_adamw_tensor* tensors, int count, Scalars s, int* 
         const int n = count - lo < kMaxTensors ? count - lo : kMaxTensors;
         uint32_t blocks = 0;
         // a small step has small arguments: 6 tensors 10.6 us, with room for kMaxTensors 14.7 us
-        cudaError_t e = n <= 16 ? go(std::integral_constant<int, 16>{}, lo, n, &blocks)
-                                : go(std::integral_constant<int, kMaxTensors>{}, lo, n, &blocks);
+        cudaError_t e = n <= 16   ? go(std::integral_constant<int, 16>{}, lo, n, &blocks)
+                        : n <= 64 ? go(std::integral_constant<int, 64>{}, lo, n, &blocks)
+                                  : go(std::integral_constant<int, kMaxTensors>{}, lo, n, &blocks);
         if (e != cudaSuccess) return e;
         s.block0 += blocks;
     }

@@ -5,10 +5,8 @@ travel as kernel arguments, so a step needs no copies and no host synchronisatio
 CUDA graph (a replay repeats the captured step number).
 """
 import ctypes
-from operator import attrgetter
 from typing import Optional
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -64,12 +62,9 @@ class AdamW:
                     d.v, d.m_scale, d.v_scale = (s[k].data_ptr() for k in ("exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale"))
                 if self.master and dtype != torch.float32:
                     d.master = s["master"].data_ptr()
-            # the descriptors' columns that a step writes, as one array each
-            fields = np.frombuffer(desc, dtype=np.dtype(_lib.AdamWTensor))
-            shapes = [self.params[i].shape for i in at]
-            self._groups.append((dtype, at, shapes, fields["n"].copy(), desc, list(desc), fields["grad"], fields["n"]))
+            self._groups.append((dtype, [(i, d, self.params[i].shape, d.n) for i, d in zip(at, desc)], desc))
         self._config = _lib.AdamWConfig(state_bits=state_bits)
-        self._partial = False  # the last step left some tensors out
+        self._partial = False  # a step has left tensors out by n = 0
 
     def _states(self, given) -> dict:
         P = self.params
@@ -109,38 +104,32 @@ class AdamW:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != self.dev):
             raise ValueError(f"grad_scale must be one float32 on {self.dev}")
-        keep, calls = [], []  # keep: copies of gradients that were not contiguous
-        partial = False
-        for dtype, at, shapes, sizes, desc, each, grad_field, n_field in self._groups:
-            mine = grads if len(at) == len(grads) else [grads[i] for i in at]
-            given = [g for g in mine if g is not None]
-            if not given:
-                continue
-            kinds = set(map(attrgetter("dtype"), given))
-            gdtype = kinds.pop()
-            if kinds or (gdtype != dtype and gdtype != torch.float32):
-                raise ValueError(f"gradients of {dtype} parameters must all be {dtype} or all float32, not {gdtype} {list(kinds)}")
-            all_given = len(given) == len(at)
-            if list(map(attrgetter("shape"), given)) != (shapes if all_given else [s for s, g in zip(shapes, mine) if g is not None]) \
-                    or set(map(torch.Tensor.get_device, given)) != {self.dev.index}:
-                raise ValueError("every gradient must have its parameter's shape and device")
-            if not all(map(torch.Tensor.is_contiguous, given)):
-                given = [g.contiguous() for g in given]
-                keep.append(given)
-            if all_given:
-                if len(each) <= 12:  # an array's assignment costs as much as twelve fields'
-                    for d, g in zip(each, given):
-                        d.grad = g.data_ptr()
-                else:
-                    grad_field[:] = list(map(torch.Tensor.data_ptr, given))
+        keep = []  # copies of gradients that were not contiguous
+        calls = []
+        index = self.dev.index
+        for dtype, tensors, desc in self._groups:
+            gdtype = None
+            for i, d, shape, n in tensors:
+                g = grads[i]
+                if g is None:
+                    d.n, self._partial = 0, True
+                    continue
+                if g.dtype is not gdtype:
+                    if gdtype is not None:
+                        raise ValueError(f"gradient {i} is {g.dtype}, others of {dtype} parameters are {gdtype}")
+                    gdtype = g.dtype
+                    if gdtype != dtype and gdtype != torch.float32:
+                        raise ValueError(f"gradient {i} must be {dtype} or float32, not {gdtype}")
+                if g.shape != shape or g.get_device() != index:
+                    raise ValueError(f"gradient {i} must have its parameter's shape and device")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    keep.append(g)
+                d.grad = g.data_ptr()
                 if self._partial:
-                    n_field[:] = sizes
-            else:
-                there = np.array([g is not None for g in mine])
-                grad_field[there], n_field[:] = list(map(torch.Tensor.data_ptr, given)), sizes * there
-                partial = True
-            calls.append((_DTYPES[dtype], _DTYPES[gdtype], desc))
-        self._partial = partial
+                    d.n = n
+            if gdtype is not None:
+                calls.append((_DTYPES[dtype], _DTYPES[gdtype], desc))
         t, c = self.step_count + 1, self._config
         c.step, c.lr = t, self.lr if lr is None else lr
         c.beta1, c.beta2 = self.betas
