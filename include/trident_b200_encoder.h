@@ -107,7 +107,7 @@ typedef struct trident_adamw_config {
  * in 32 bits. 8-bit states are decoded, updated and used in 32 bits, then encoded again with the scale
  * max / 448 of their block: m to the nearest value; sqrt(v) at random to one of its two neighbours so
  * that its mean is kept (to the nearest, the 1 - beta2 of a typical step would always round away), and
- * never to 0 unless v is below 2^-126. The random bits are a hash of rounding_seed and the element's place, counted
+ * never to 0 unless v is 0. The random bits are a hash of rounding_seed and the element's place, counted
  * in whole blocks over the tensors in order. A block with a NaN or infinite state has a scale that is
  * not finite. Tensors must not overlap; n = 0 is allowed. */
 int trident_adamw_step(const trident_adamw_tensor* tensors, int32_t count, const trident_adamw_config* config,

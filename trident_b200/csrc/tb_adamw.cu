@@ -8,9 +8,10 @@
 //
 // 32-bit states are bound by their bytes: 40M bf16 values with master copies (28 bytes a value) take 169 us on
 // a B200, 6.6 TB/s. Thread blocks come in order and none stays: a resident grid that strides over the tensors
-// took 206 us. 8-bit states (10 bytes a value) need about 330 instructions for a lane's 8 values: 100M bf16 values
-// take 188 us, 5.3 TB/s, with five thread blocks an SM (48 registers; 197 us with four). Packed float pairs and
-// approximate roots and reciprocals brought 382 to 213 us, the scales' lines of their own 213 to 197 us.
+// took 206 us. 8-bit states (10 bytes a value) are bound by instructions, some 380 for a lane's 8 values: 100M
+// bf16 values take 223 us, 4.5 TB/s. Packed float pairs brought 382 us to 213, the scales' lines of their own
+// that to 188; the moments' separate roundings and the exact square root, without which the 8-bit values of two
+// machines part in a few places of a million, cost 35 us of it.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -139,12 +140,9 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, int n, uint2 w) {
 }
 
 // What a block of maximum `top` is multiplied by before its encoding, and its scale. A maximum below kTiny
-// counts as 0, as its reciprocal would overflow; that of a maximum above 2^126 would be flushed to 0.
-__device__ __forceinline__ float encoding_factor(float top) {
-    if (top < kTiny) return 0.0f;
-    return top < 1e30f ? kE4m3Max * rcp_approx(top) : kE4m3Max / top;
-}
-__device__ __forceinline__ float block_scale(float top) { return top < kTiny ? 0.0f : top * (1.0f / kE4m3Max); }
+// counts as 0, as its reciprocal would overflow.
+__device__ __forceinline__ float encoding_factor(float top) { return top < kTiny ? 0.0f : __fdiv_rn(kE4m3Max, top); }
+__device__ __forceinline__ float block_scale(float top) { return top < kTiny ? 0.0f : __fdiv_rn(top, kE4m3Max); }
 
 // An 8-bit state's encoding: scaled by mul to the block's maximum. m: to nearest.
 __device__ __forceinline__ uint2 encode_nearest(const float2* v, float mul) {
@@ -176,9 +174,9 @@ __device__ __forceinline__ uint2 encode_random(const float2* v, float mul, uint3
 }
 
 template <class P, class G, bool MASTER, bool BITS8, int CAP>
-__global__ void __launch_bounds__(256, BITS8 ? 5 : 4) adamw_kernel(const __grid_constant__ Tensors<CAP> a) {
+__global__ void __launch_bounds__(256, 4) adamw_kernel(const __grid_constant__ Tensors<CAP> a) {
     constexpr int UNIT = kUnit<BITS8>;
-    __shared__ float scales[2][UNIT];  // of m and of v's root: the old ones, then the new
+    __shared__ float scales[2][UNIT];  // of m and of v's root: the old scales, then the new maxima
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t u = blockIdx.x;
     const float gs = a.s.grad_scale ? *a.s.grad_scale : 1.0f;
@@ -233,9 +231,10 @@ __global__ void __launch_bounds__(256, BITS8 ? 5 : 4) adamw_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 gi = __fmul2_rn(g[i], splat(gs));
-            m[i] = __ffma2_rn(gi, splat(a.s.keep1), __fmul2_rn(m[i], splat(a.s.beta1)));
-            v[i] = __ffma2_rn(__fmul2_rn(gi, gi), splat(a.s.keep2), __fmul2_rn(v[i], splat(a.s.beta2)));
-            root[i] = make_float2(sqrt_approx(v[i].x), sqrt_approx(v[i].y));
+            // each operation rounded by itself: what is encoded in 8 bits is the formula's, to the last bit
+            m[i] = add2_apart(__fmul2_rn(m[i], splat(a.s.beta1)), __fmul2_rn(gi, splat(a.s.keep1)));
+            v[i] = add2_apart(__fmul2_rn(v[i], splat(a.s.beta2)), __fmul2_rn(__fmul2_rn(gi, gi), splat(a.s.keep2)));
+            root[i] = BITS8 ? make_float2(__fsqrt_rn(v[i].x), __fsqrt_rn(v[i].y)) : make_float2(sqrt_approx(v[i].x), sqrt_approx(v[i].y));
             const float2 denom = __ffma2_rn(root[i], splat(a.s.inv_root), splat(a.s.eps));
             const float2 upd = __fmul2_rn(__fmul2_rn(m[i], splat(a.s.step_size)), make_float2(rcp_approx(denom.x), rcp_approx(denom.y)));
             p[i] = __ffma2_rn(p[i], splat(a.s.decay), upd);
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(256, BITS8 ? 5 : 4) adamw_kernel(const __grid_
             const bool small = !(warp_min(root) * mul >= kE4m3Min);
             store_bytes<WHOLE>(static_cast<uint8_t*>(t.v) + at, n,
                                small ? encode_random<true>(root, mul, pair, a.s.seed) : encode_random<false>(root, mul, pair, a.s.seed));
-            if (lane < 2) scales[lane][k] = block_scale(lane ? vt : mt);
+            if (lane < 2) scales[lane][k] = lane ? vt : mt;
         } else {
             store_lane<float, WHOLE>(static_cast<float*>(t.m) + at, n, m);
             store_lane<float, WHOLE>(static_cast<float*>(t.v) + at, n, v);
@@ -272,7 +271,7 @@ __global__ void __launch_bounds__(256, BITS8 ? 5 : 4) adamw_kernel(const __grid_
         __syncthreads();
         if (threadIdx.x < 2 * UNIT && (threadIdx.x & (UNIT - 1)) < there) {
             const int i = threadIdx.x & (UNIT - 1);
-            (threadIdx.x < UNIT ? t.m_scale : t.v_scale)[block0 + i] = scales[threadIdx.x / UNIT][i];
+            (threadIdx.x < UNIT ? t.m_scale : t.v_scale)[block0 + i] = block_scale(scales[threadIdx.x / UNIT][i]);
         }
     }
 }

@@ -98,6 +98,10 @@ struct Pack {
 // Packed pairs of floats: one instruction for two operations.
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
 
+// The sum of two products of pairs with each product rounded. (Packed, the compiler joins a product and a sum
+// into one fused operation, whatever rounding they name; single sums of packed products stay apart.)
+__device__ __forceinline__ float2 add2_apart(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+
 // The 16 bytes at p as pairs of floats (4 of float32, 8 of a 16-bit type), and back.
 template <class T> constexpr int kPairs16 = 8 / (int)sizeof(T);
 template <class T>
