@@ -40,8 +40,8 @@ int trident_embed_grad_workspace_size(int64_t T, int64_t V, int32_t D, size_t* b
 
 /* The lookup's gradient: out[v, :] = scale * sum over t with ids[t] = v of grad[t, :], or that sum added
  * to out[v, :] (accumulate = 1; rows that no id names are then not touched). Ids outside [0, V) give
- * nothing (-1 silently, others set TRIDENT_STATUS_BAD_ID). Each row's sum is taken over t in ascending
- * order, in pieces that depend on the ids alone, in 32 bits, and rounded once.
+ * nothing (-1 silently, others set TRIDENT_STATUS_BAD_ID). Each row's sum is taken in an order that the
+ * ids alone fix, in 32 bits, and rounded once.
  *   grad [T, D] of `dtype`; out [V, D] of out_dtype (`dtype` or TRIDENT_F32); T, V < 2^31; the workspace
  *   is 256-byte aligned. */
 int trident_embed_grad(const void* grad, int32_t dtype, int64_t ld_grad, const void* ids, int32_t id_bits, int64_t T,

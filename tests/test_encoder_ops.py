@@ -533,3 +533,37 @@ def test_operators_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_zeros_beside_the_sort_on_streams_and_in_a_graph():
+    """A gradient whose zeros are written on the library's second stream: on a side stream, with the output used at
+    once after the call, and captured."""
+    import torch
+
+    import trident_b200 as tb
+
+    V, D, T = 30_000, 256, 5000
+    ids, grad = _ids(T, V, 1), _randn((T, D), "bfloat16", 2)
+    want, mag, count = _grad_reference(grad, ids, V, 1.0)
+    tol = _grad_tol(want, mag, count, "bfloat16")
+    out = torch.full((V, D), 3.0, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            out.fill_(3.0)
+            tb.embedding_grad(grad, ids, V, out=out)
+            used = out * 1.0
+    side.synchronize()
+    _close(used, want, tol)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        tb.embedding_grad(grad, ids, V, out=out)
+        used = out * 1.0
+    for seed in (3, 4):
+        grad.copy_(_randn((T, D), "bfloat16", seed))
+        out.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want, mag, count = _grad_reference(grad, ids, V, 1.0)
+        _close(used, want, _grad_tol(want, mag, count, "bfloat16"))

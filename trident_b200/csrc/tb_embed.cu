@@ -800,6 +800,20 @@ bool cluster_fits() {
 // ids in place of 33 us; 61 MB, 35 in place of 45 us.
 constexpr int64_t kSideZeros = 4 << 20;
 
+// Work on the side stream that the caller's stream has to wait for, whichever way the call ends.
+struct Beside {
+    SideStream* ss;
+    cudaStream_t st;
+    cudaError_t join() {
+        if (!ss) return cudaSuccess;
+        SideStream* s = ss;
+        ss = nullptr;
+        const cudaError_t e = cudaEventRecord(s->join, s->s);
+        return e != cudaSuccess ? e : cudaStreamWaitEvent(st, s->join, 0);
+    }
+    ~Beside() { join(); }
+};
+
 template <class T, class O>
 cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int64_t count, int64_t V, int D, float scale,
                        int accumulate, O* out, int64_t ld_out, void* workspace, int32_t* status, int* launches,
@@ -807,20 +821,21 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
     cudaError_t e;
     constexpr int kMax = 16 / (int)sizeof(T);
     int vec = wide_elements({{grad, ld, (int)sizeof(T)}, {out, ld_out, (int)sizeof(O)}}, D, kMax);
-    SideStream* side = nullptr;  // zeros are written beside the sort
+    Beside side{nullptr, st};  // zeros are written beside the sort
     if (!accumulate && V > 0) {
         const int64_t row_bytes = (int64_t)D * sizeof(O);
         cudaStream_t zs = st;
         if (count > kDirectIds && V * row_bytes >= kSideZeros) {
-            if ((e = side_stream(&side)) != cudaSuccess) return e;
-            if ((e = cudaEventRecord(side->fork, st)) != cudaSuccess) return e;
-            if ((e = cudaStreamWaitEvent(side->s, side->fork, 0)) != cudaSuccess) return e;
-            zs = side->s;
+            SideStream* ss = nullptr;
+            if ((e = side_stream(&ss)) != cudaSuccess) return e;
+            if ((e = cudaEventRecord(ss->fork, st)) != cudaSuccess) return e;
+            if ((e = cudaStreamWaitEvent(ss->s, ss->fork, 0)) != cudaSuccess) return e;
+            side.ss = ss;
+            zs = ss->s;
         }
         e = ld_out == D ? cudaMemsetAsync(out, 0, (size_t)V * row_bytes, zs)
                         : cudaMemset2DAsync(out, ld_out * sizeof(O), 0, (size_t)row_bytes, V, zs);
         if (e != cudaSuccess) return e;
-        if (side && (e = cudaEventRecord(side->join, side->s)) != cudaSuccess) return e;
     }
     if (count == 0) return cudaSuccess;
     if (count <= kDirectIds) {
@@ -875,7 +890,8 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
         }
         *launches += 2 * passes;
     }
-    if (side && (e = cudaStreamWaitEvent(st, side->join, 0)) != cudaSuccess) return e;
+    const bool joined = side.ss != nullptr;
+    if ((e = side.join()) != cudaSuccess) return e;
     RunArgs a;
     a.items = ws.items[(passes - 1) & 1];
     a.count = count;
@@ -897,7 +913,7 @@ cudaError_t grad_typed(const T* grad, int64_t ld, const void* ids, int id64, int
         auto go = [&](auto l) {
             constexpr int LANES = decltype(l)::value;
             const auto sum = accumulate ? run_sum_kernel<T, O, VEC, LANES, true> : run_sum_kernel<T, O, VEC, LANES, false>;
-            if (side) {
+            if (joined) {
                 sum<<<(unsigned)grid, 256, 0, st>>>(a, grad, out);
                 e = cudaGetLastError();
             } else {

@@ -123,7 +123,7 @@ def embedding_lookup(table, ids, scale: float = 1.0, out=None, status=None):
 def embedding_grad(grad_out, ids, num_rows: int, scale: float = 1.0, out=None, accumulate: bool = False,
                    dtype: Optional[torch.dtype] = None, status=None):
     """The gradient of embedding_lookup with respect to its table: [num_rows, D], row v being scale times the
-    sum of grad_out's rows whose id is v, in the order of the ids.
+    sum of grad_out's rows whose id is v, in an order that the ids alone fix.
 
     grad_out: [*ids.shape, D]. Ids outside [0, num_rows) give nothing (all but -1 set `status`, as in the
     lookup). dtype: that of grad_out (default) or float32. out: a tensor to write to; with accumulate=True
