@@ -59,7 +59,6 @@ struct Pack {
         return r;
     }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
-    __device__ __forceinline__ void store_stream(T* p) const { __stcs(reinterpret_cast<Raw*>(p), raw); }
 
     __device__ __forceinline__ void get(float* f) const {
         if constexpr (N == 1) {
